@@ -31,7 +31,8 @@ page and head: key codes, key groups, value codes, value groups.
   value of a code: (code - 8) * scale + centre, per token and group of G
   group word:  [D / G, P], scale in the low 16 bits, centre in the high (fp16)
   key codes:   [P, D / 8]: values 8o..8o+7 in the word (D / 32) * (o % 4) + o // 4
-  value codes: [P / 8, D]: eight tokens of one value in a word
+  value codes: [P / 8, D]: eight tokens of value d in the word 64 * (d // 64)
+               + 4 * (d % 16) + d // 16 % 4
   the i-th of eight codes in a word lies in bits [4n, 4n + 4), n = i // 2 + 4 * (i % 2)
 """
 from __future__ import annotations
@@ -256,6 +257,12 @@ def _octet_order(D: int, device) -> torch.Tensor:
     return (w % (D // 32)) * 4 + w // (D // 32)
 
 
+def _value_order(D: int, device) -> torch.Tensor:
+    """In which word of its row each value lies."""
+    d = torch.arange(D, device=device)
+    return 64 * (d // 64) + 4 * (d % 16) + d // 16 % 4
+
+
 def _group_words(s: torch.Tensor, c: torch.Tensor) -> torch.Tensor:
     return torch.stack((s, c), -1).view(torch.int32).squeeze(-1)
 
@@ -267,6 +274,7 @@ def _pack(k: torch.Tensor, v: torch.Tensor, G: int) -> torch.Tensor:
     vc, vs, vz = _groups(v, G)
     kw = _words(kc.view(n, H, P, D // 8, 8))[..., _octet_order(D, k.device)]
     vw = _words(vc.view(n, H, P // 8, 8, D).transpose(-1, -2))
+    vw = vw[..., torch.argsort(_value_order(D, k.device))]
     parts = (kw, _group_words(ks, kz).transpose(-1, -2), vw, _group_words(vs, vz).transpose(-1, -2))
     return torch.cat([p.reshape(n, H, -1) for p in parts], -1)
 
@@ -297,7 +305,8 @@ def _unpack(blocks: torch.Tensor, case: dict) -> tuple[torch.Tensor, torch.Tenso
     kw = blocks[..., :a].reshape(*lead, P, D // 8)
     kw = kw[..., torch.argsort(_octet_order(D, blocks.device))]
     kc = _unwords(kw).reshape(*lead, P, D)
-    vc = _unwords(blocks[..., b:c].reshape(*lead, P // 8, D)).transpose(-1, -2)
+    vw = blocks[..., b:c].reshape(*lead, P // 8, D)[..., _value_order(D, blocks.device)]
+    vc = _unwords(vw).transpose(-1, -2)
     vc = vc.reshape(*lead, P, D)
     k = _ungroup(kc, blocks[..., a:b].reshape(*lead, D // G, P).transpose(-1, -2), G)
     v = _ungroup(vc, blocks[..., c:d].reshape(*lead, D // G, P).transpose(-1, -2), G)
@@ -485,7 +494,7 @@ def _append_plain(state: dict):
     flat[at + a + groups + tok] = _group_words(ks, kz)
     flat[at + c + groups + tok] = _group_words(vs, vz)
     # eight tokens share a word: every token adds its own change to it
-    word = at + b + tok // 8 * D + torch.arange(D, device=_DEVICE)
+    word = at + b + tok // 8 * D + _value_order(D, _DEVICE)
     i = tok % 8
     shift = (4 * (i // 2 + 4 * (i % 2))).to(torch.int32)
     old = (flat[word] >> shift) & 15
@@ -508,7 +517,7 @@ def _read_plain(state: dict):
     kc = _unwords(flat[at + tok * (D // 8) + order]).flatten(-2)
     i = tok % 8
     shift = (4 * (i // 2 + 4 * (i % 2))).to(torch.int32)
-    vc = (flat[at + b + tok // 8 * D + torch.arange(D, device=_DEVICE)] >> shift) & 15
+    vc = (flat[at + b + tok // 8 * D + _value_order(D, _DEVICE)] >> shift) & 15
     groups = torch.arange(D // G, device=_DEVICE) * P
     return (_ungroup(kc, flat[at + a + groups + tok], G),
             _ungroup(vc, flat[at + c + groups + tok], G))
@@ -678,7 +687,8 @@ def _stored(pool: torch.Tensor, pages: torch.Tensor, head: int, case: dict):
     meta = block[:, at + d // G * P + t]
     k = k * _half(meta) + _half(meta >> 16)
     at += P * (D // G)
-    v = _code(block[:, at + t // 8 * D + d], (t % 8).expand(P, D)).double() - 8
+    vword = d - d % 64 + d % 16 * 4 + d % 64 // 16
+    v = _code(block[:, at + t // 8 * D + vword], (t % 8).expand(P, D)).double() - 8
     at += P * D // 8
     meta = block[:, at + d // G * P + t]
     v = v * _half(meta) + _half(meta >> 16)

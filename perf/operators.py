@@ -461,7 +461,9 @@ def _rotate(x: torch.Tensor, w, state: dict) -> torch.Tensor:
         t = t[..., 0] + t[..., 1]
         while t.shape[-1] > 1:
             t = t[..., :t.shape[-1] // 2] + t[..., t.shape[-1] // 2:]
-        x = x * (1.0 / torch.sqrt(t * (1.0 / D) + _EPS)) * w.float()
+        # (torch's fp32 square root is not rounded correctly; by way of fp64 it is)
+        root = (t * (1.0 / D) + _EPS).double().sqrt().float()
+        x = x * (1.0 / root) * w.float()
     R, pos = case["R"], state["positions"].long()
     c, s = state["cos"][pos][:, None], state["sin"][pos][:, None]
     if case["inter"]:

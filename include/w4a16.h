@@ -291,6 +291,164 @@ int w4a16_unpack_int4(const int32_t* qweight, int32_t* q, int64_t K, int64_t N, 
 int w4a16_dequantize_f16(const int32_t* qweight, const void* scales, const void* zeros, void* w,
                          int64_t K, int64_t N, int64_t group_size, void* stream);
 
+/* ---- 4-bit paged key / value cache ------------------------------------------
+ *
+ * What an attention layer needs between its projections.  No reference
+ * counterpart (the reference is the GEMM alone).  A pool holds pages of P tokens
+ * for every layer; one layer's pool is int32 [pages, heads, words] with
+ *   words = P * (D / 4 + 2 * D / G)                      (w4a16_kv4_words)
+ * and a block of words holds, in this order, key codes [P, D/8], key groups
+ * [D/G, P], value codes [P/8, D], value groups [D/G, P]:
+ *   value = (code - 8) * scale + centre     code 0..15, G values of one token
+ *                                           share a scale and a centre
+ *   group word: fp16 scale in the low 16 bits, fp16 centre in the high
+ *   the i-th of a word's eight codes lies in bits [4n, 4n+4), n = i/2 + 4*(i%2)
+ *   keys: values 8o..8o+7 of a token in word (D/32) * (o % 4) + o/4 of its row
+ *   values: value d of tokens 8u..8u+7 in word 64*(d/64) + 4*(d%16) + d/16 % 4
+ * A group of numbers lo..hi is stored with scale = fp16((hi - lo) / 15), centre =
+ * fp16(lo + 8 * scale), code = clamp(rint((x - centre) * (1 / scale)), -8, 7) + 8
+ * (fp32, round to even); 8 where the scale is 0 or not finite.
+ *
+ * A page table is int32 [rows, max_pages]: one row per sequence, page ids in the
+ * order of its tokens, -1 where there is none.  Row, position and page ids that
+ * lie outside their tensors are never followed.
+ *
+ * D is 64, 128 or 256; G is D, D/2 or D/4 and at least 32; P is 32, 64, 128 or
+ * 256.  Calls launch kernels only and can be captured into a HIP graph.
+ */
+
+/* flags of the calls below */
+#define W4A16_KV4_BF16 1        /* queries, keys, values, weights, results: bf16, else fp16 */
+#define W4A16_KV4_INTERLEAVED 2 /* values 2i, 2i+1 rotate together, else i, i + rot_dim/2 */
+#define W4A16_KV4_CAUSAL 4      /* a query sees no later position than its own    */
+
+/* New tokens: q [tokens, q_heads, head_dim] and k, v [tokens, kv_heads, head_dim]
+ * of any token and head strides (elements), unit stride inside a head. */
+typedef struct w4a16_rope {
+  const void *q, *k, *v;       /* v: w4a16_kv4_append only                       */
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head;
+  void* q_out;                 /* [tokens, q_heads, head_dim], contiguous        */
+  void* k_out;                 /* [tokens, kv_heads, head_dim]; w4a16_qk_norm_rope only */
+  const float *cos, *sin;      /* fp32 [positions, rot_dim / 2], contiguous      */
+  const int32_t* token_position; /* [tokens]                                     */
+  const void *q_weight, *k_weight; /* [head_dim]; NULL: that side is not normed  */
+  int64_t tokens, positions;
+  int32_t q_heads, kv_heads, head_dim;
+  int32_t rot_dim;             /* rotated values of a head: a multiple of 16     */
+  float eps;
+  int32_t flags;               /* W4A16_KV4_BF16 | W4A16_KV4_INTERLEAVED         */
+} w4a16_rope;
+
+/* One layer's pool with the page table that leads into it. */
+typedef struct w4a16_kv4 {
+  int32_t* pool;               /* [pages, heads, words], 16-byte aligned         */
+  const int32_t* table;        /* [rows, max_pages]                              */
+  int64_t pages, rows, max_pages;
+  int32_t heads, head_dim, group_size, page_size;
+} w4a16_kv4;
+
+/* Queries of one attention call. */
+typedef struct w4a16_kv4_query {
+  const void* q;               /* [tokens, q_heads, head_dim], strides in elements */
+  int64_t q_token, q_head;
+  void* out;                   /* [tokens, q_heads, head_dim], contiguous        */
+  float* lse;                  /* [tokens, q_heads] or NULL                      */
+  const int32_t* lens;         /* [rows of the table]: tokens stored             */
+  const int32_t* q_starts;     /* [batch + 1], or NULL: one token a sequence     */
+  const int32_t* seqs;         /* [batch] table row of each, or NULL: row b      */
+  int64_t tokens, batch, max_q, max_context;
+  int32_t q_heads;
+  int32_t window;              /* last positions a query sees; 0: all            */
+  float scale;
+  int32_t flags;               /* W4A16_KV4_BF16 | W4A16_KV4_CAUSAL              */
+} w4a16_kv4_query;
+
+/* The page bookkeeping of a pool, all on the device. */
+typedef struct w4a16_kv4_book {
+  int32_t* table;              /* [rows, max_pages]                              */
+  int32_t* lens;               /* [rows]                                         */
+  int32_t* refs;               /* [pages]: rows that hold the page               */
+  int64_t rows, max_pages, pages;
+  int32_t page_size;
+} w4a16_kv4_book;
+
+/* bits that the page calls set in *status (a device int32 that keeps them) */
+#define W4A16_KV4_NO_PAGES 1 /* the pool had no free page: that row is unchanged  */
+#define W4A16_KV4_ROW_FULL 2 /* more than max_pages: that row is unchanged        */
+#define W4A16_KV4_BAD_ROW 4  /* no such row, a negative count, or a child in use  */
+
+/* Words of one page and head, or a negative w4a16_status. */
+int64_t w4a16_kv4_words(int32_t head_dim, int32_t group_size, int32_t page_size);
+
+/*
+ * Queries and keys per head: y = x / sqrt(mean(x^2) + eps) * weight, then the
+ * rotation of their first rot_dim values by their token's position; fp32, rounded
+ * once.  The squares are summed in one fixed order, so a token's results do not
+ * depend on the tokens beside it.  A token whose position lies outside the tables
+ * gets NaN.
+ */
+int w4a16_qk_norm_rope(const w4a16_rope* t, void* stream);
+
+/*
+ * The same, the keys (quantised from fp32) and the values stored at their token's
+ * position of table row rows[i] (row i where rows is NULL) instead of written.  A
+ * token with a negative position, or one that the tables do not hold, is not
+ * stored.  Two tokens of one call must not have the same place.
+ */
+int w4a16_kv4_append(const w4a16_rope* t, const w4a16_kv4* kv, const int32_t* rows, void* stream);
+
+/* Stored tokens as [tokens, heads, head_dim] (flags: W4A16_KV4_BF16); zeros for a
+ * place that the table does not hold. */
+int w4a16_kv4_read(const w4a16_kv4* kv, const int32_t* token_position, const int32_t* rows,
+                   int64_t tokens, void* k, void* v, int32_t flags, void* stream);
+
+/* Device workspace of w4a16_kv4_attention (0 = none): fp32 partial results. */
+size_t w4a16_kv4_attention_workspace_bytes(const w4a16_kv4* kv, const w4a16_kv4_query* q);
+
+/*
+ * Attention of each sequence's new tokens over its stored ones (the new ones among
+ * them).  Sequence b has tokens q_starts[b] .. q_starts[b+1] - 1 of q, its last ones;
+ * query i of nq stands at position lens - nq + i and sees the positions t < lens
+ * with t <= its own (W4A16_KV4_CAUSAL) and t > its own - window (window > 0).
+ * A query that sees nothing gets zeros and lse = -inf.  q_heads is a multiple of
+ * heads; query head j uses head j / (q_heads / heads).  max_q bounds the tokens a
+ * sequence has in q (it has no more than this: the rest is not computed);
+ * max_context only sizes the launch (any length is right, the largest is fast).
+ * The workspace (256-byte aligned, w4a16_kv4_attention_workspace_bytes) needs no
+ * initialisation; calls that share one must be ordered.
+ */
+int w4a16_kv4_attention(const w4a16_kv4* kv, const w4a16_kv4_query* q, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/*
+ * Pages.  `pool` is int32 [layers, pages, page_words], page_words = heads * words.
+ * Pages are taken lowest first, in the order of the lists.
+ *
+ * copy_pages: page src[i] to page dst[i] in every layer; no dst is another's src
+ * or dst.  Pairs outside the pool are skipped.
+ * extend: row seqs[i] gets room for counts[i] more tokens and its length grows by
+ * them (a row is named once).
+ * fork: row children[i] (empty) becomes a copy of row parents[i]: whole pages are
+ * shared, a partly filled last page is copied to one of its own.
+ * free: rows seqs[i] are emptied; pages that no other row holds become free.
+ * compact: pages in use move to the front of the pool, the k-th that lies beyond
+ * the number in use to the k-th free one before it; new_table and new_refs say
+ * where they are now, *live how many are in use.
+ */
+int w4a16_kv4_copy_pages(int32_t* pool, int64_t layers, int64_t pages, int64_t page_words,
+                         const int32_t* src, const int32_t* dst, int64_t n, void* stream);
+int w4a16_kv4_extend(const w4a16_kv4_book* book, const int32_t* seqs, const int32_t* counts,
+                     int64_t n, int32_t* status, void* stream);
+size_t w4a16_kv4_fork_workspace_bytes(int64_t n);
+int w4a16_kv4_fork(int32_t* pool, int64_t layers, int64_t page_words, const w4a16_kv4_book* book,
+                   const int32_t* parents, const int32_t* children, int64_t n, int32_t* status,
+                   void* workspace, size_t workspace_bytes, void* stream);
+int w4a16_kv4_free(const w4a16_kv4_book* book, const int32_t* seqs, int64_t n, void* stream);
+size_t w4a16_kv4_compact_workspace_bytes(int64_t pages);
+int w4a16_kv4_compact(int32_t* pool, int64_t layers, int64_t page_words,
+                      const w4a16_kv4_book* book, int32_t* new_table, int32_t* new_refs,
+                      int32_t* live, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

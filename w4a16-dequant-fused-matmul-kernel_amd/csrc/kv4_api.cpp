@@ -1,0 +1,223 @@
+// C entry points of the 4-bit paged cache: arguments are checked here, on the
+// host, before anything is launched.
+#include "kv4_launch.h"
+
+namespace w4a16 {
+namespace {
+
+constexpr int64_t kMax = INT32_MAX;
+bool size_ok(int64_t n) { return n >= 0 && n <= kMax; }
+bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+hipStream_t stream_of(void* s) { return static_cast<hipStream_t>(s); }
+
+int head_check(int32_t D) { return D == 64 || D == 128 || D == 256 ? W4A16_OK : W4A16_ERR_BAD_SHAPE; }
+int page_check(int32_t P) {
+  return P >= 32 && P <= 256 && (P & (P - 1)) == 0 ? W4A16_OK : W4A16_ERR_BAD_SHAPE;
+}
+int geometry_check(int32_t D, int32_t G, int32_t P) {
+  if (int e = head_check(D)) return e;
+  if (int e = page_check(P)) return e;
+  return G >= 32 && (G == D || 2 * G == D || 4 * G == D) ? W4A16_OK : W4A16_ERR_BAD_GROUP;
+}
+
+int kv_check(const w4a16_kv4& kv) {
+  if (int e = geometry_check(kv.head_dim, kv.group_size, kv.page_size)) return e;
+  if (kv.heads < 1 || kv.heads > 65535 || !size_ok(kv.pages) || !size_ok(kv.rows) ||
+      !size_ok(kv.max_pages))
+    return W4A16_ERR_BAD_SHAPE;
+  if ((kv.pages && !kv.pool) || (kv.rows && kv.max_pages && !kv.table)) return W4A16_ERR_NULL_POINTER;
+  return aligned(kv.pool, 16) && aligned(kv.table, 4) ? W4A16_OK : W4A16_ERR_BAD_PLAN;
+}
+
+int rope_check(const w4a16_rope& t, bool store) {
+  const int known = W4A16_KV4_BF16 | W4A16_KV4_INTERLEAVED;
+  if (t.flags & ~known) return W4A16_ERR_BAD_PLAN;
+  if (int e = head_check(t.head_dim)) return e;
+  if (t.q_heads < 0 || t.kv_heads < 0 || !size_ok(t.tokens) || !size_ok(t.positions) ||
+      t.rot_dim < 0 || t.rot_dim > t.head_dim || t.rot_dim % 16 ||
+      t.tokens * ((int64_t)t.q_heads + t.kv_heads) > kMax)
+    return W4A16_ERR_BAD_SHAPE;
+  if (t.tokens == 0) return W4A16_OK;
+  const bool has_q = t.q_heads > 0, has_k = t.kv_heads > 0;
+  if (!t.token_position || (has_q && (!t.q || !t.q_out)) || (has_k && !t.k) ||
+      (has_k && (store ? !t.v : !t.k_out)) ||
+      (t.rot_dim && t.positions && (!t.cos || !t.sin)))
+    return W4A16_ERR_NULL_POINTER;
+  // results are stored 16 bytes at a time, inputs read so where they allow it
+  if (!aligned(t.q_out, 16) || !aligned(t.k_out, 16) || !aligned(t.q, 2) || !aligned(t.k, 2) ||
+      !aligned(t.v, 2))
+    return W4A16_ERR_BAD_PLAN;
+  return W4A16_OK;
+}
+
+int query_check(const w4a16_kv4& kv, const w4a16_kv4_query& q) {
+  if (int e = kv_check(kv)) return e;
+  if (q.flags & ~(W4A16_KV4_BF16 | W4A16_KV4_CAUSAL)) return W4A16_ERR_BAD_PLAN;
+  if (q.q_heads < 1 || q.q_heads % kv.heads || !size_ok(q.tokens) || !size_ok(q.batch) ||
+      !size_ok(q.max_q) || !size_ok(q.max_context) || q.window < 0 || !(q.scale > 0.0f) ||
+      !(q.scale < 3.0e38f) || q.tokens * (int64_t)q.q_heads > kMax)
+    return W4A16_ERR_BAD_SHAPE;
+  return !q.q_starts && q.tokens != q.batch ? W4A16_ERR_BAD_SHAPE : W4A16_OK;
+}
+
+// The launch-sizing numbers as far as the tensors can need them.
+w4a16_kv4_query bounded(const w4a16_kv4& kv, w4a16_kv4_query q) {
+  if (!q.q_starts) q.max_q = 1;
+  if (q.max_q < 1) q.max_q = 1;
+  if (q.max_q > q.tokens) q.max_q = q.tokens;
+  const int64_t most = kv.max_pages * kv.page_size;
+  if (q.max_context > most) q.max_context = most;
+  return q;
+}
+
+int book_check(const w4a16_kv4_book& b) {
+  if (int e = page_check(b.page_size)) return e;
+  if (!size_ok(b.rows) || !size_ok(b.max_pages) || !size_ok(b.pages)) return W4A16_ERR_BAD_SHAPE;
+  return (b.rows && (!b.lens || (b.max_pages && !b.table))) || (b.pages && !b.refs)
+             ? W4A16_ERR_NULL_POINTER
+             : W4A16_OK;
+}
+int pool_check(const void* pool, int64_t layers, int64_t pages, int64_t page_words) {
+  if (!size_ok(layers) || !size_ok(pages) || page_words < 4 || page_words > kMax || page_words % 4)
+    return W4A16_ERR_BAD_SHAPE;
+  if (layers && pages && !pool) return W4A16_ERR_NULL_POINTER;
+  return aligned(pool, 16) ? W4A16_OK : W4A16_ERR_BAD_PLAN;
+}
+constexpr int64_t kMaxList = 1 << 20;   // pairs or rows of one page call
+
+}  // namespace
+}  // namespace w4a16
+
+using namespace w4a16;
+
+extern "C" {
+
+int64_t w4a16_kv4_words(int32_t head_dim, int32_t group_size, int32_t page_size) {
+  if (int e = geometry_check(head_dim, group_size, page_size)) return e;
+  return (int64_t)page_size * (head_dim / 4 + 2 * (head_dim / group_size));
+}
+
+int w4a16_qk_norm_rope(const w4a16_rope* t, void* stream) {
+  if (!t) return W4A16_ERR_NULL_POINTER;
+  if (int e = rope_check(*t, false)) return e;
+  if (t->tokens == 0 || t->q_heads + t->kv_heads == 0) return W4A16_OK;
+  return (int)launch_rope(*t, nullptr, nullptr, stream_of(stream));
+}
+
+int w4a16_kv4_append(const w4a16_rope* t, const w4a16_kv4* kv, const int32_t* rows, void* stream) {
+  if (!t || !kv) return W4A16_ERR_NULL_POINTER;
+  if (int e = rope_check(*t, true)) return e;
+  if (int e = kv_check(*kv)) return e;
+  if (t->kv_heads != kv->heads || t->head_dim != kv->head_dim) return W4A16_ERR_BAD_SHAPE;
+  if (t->tokens == 0) return W4A16_OK;
+  return (int)launch_rope(*t, kv, rows, stream_of(stream));
+}
+
+int w4a16_kv4_read(const w4a16_kv4* kv, const int32_t* token_position, const int32_t* rows,
+                   int64_t tokens, void* k, void* v, int32_t flags, void* stream) {
+  if (!kv) return W4A16_ERR_NULL_POINTER;
+  if (int e = kv_check(*kv)) return e;
+  if (flags & ~W4A16_KV4_BF16) return W4A16_ERR_BAD_PLAN;
+  if (!size_ok(tokens) || tokens * kv->heads > kMax) return W4A16_ERR_BAD_SHAPE;
+  if (tokens == 0) return W4A16_OK;
+  if (!token_position || !k || !v) return W4A16_ERR_NULL_POINTER;
+  if (!aligned(k, 16) || !aligned(v, 16)) return W4A16_ERR_BAD_PLAN;
+  return (int)launch_kv4_read(*kv, token_position, rows, tokens, k, v, flags & W4A16_KV4_BF16,
+                              stream_of(stream));
+}
+
+size_t w4a16_kv4_attention_workspace_bytes(const w4a16_kv4* kv, const w4a16_kv4_query* q) {
+  if (!kv || !q || query_check(*kv, *q) != W4A16_OK || q->tokens == 0 || q->batch == 0) return 0;
+  return kv4_attention_plan(*kv, bounded(*kv, *q)).workspace;
+}
+
+int w4a16_kv4_attention(const w4a16_kv4* kv, const w4a16_kv4_query* q, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+  if (!kv || !q) return W4A16_ERR_NULL_POINTER;
+  if (int e = query_check(*kv, *q)) return e;
+  if (q->tokens == 0 || q->batch == 0) return W4A16_OK;
+  if (!q->q || !q->out || !q->lens) return W4A16_ERR_NULL_POINTER;
+  if (!aligned(q->out, 16) || !aligned(q->q, 2)) return W4A16_ERR_BAD_PLAN;
+  Kv4Attn a{};
+  a.kv = *kv;
+  a.q = bounded(*kv, *q);
+  const Kv4Plan p = kv4_attention_plan(a.kv, a.q);
+  const double groups = (double)kv->heads * p.splits * (double)q->batch * p.tiles;
+  const double joins = (double)q->q_heads * (double)a.q.max_q * (double)q->batch;
+  if (groups > (double)kMax || joins > (double)kMax) return W4A16_ERR_BAD_SHAPE;
+  if (p.workspace && (!workspace || workspace_bytes < p.workspace)) return W4A16_ERR_WORKSPACE;
+  if (p.workspace && !aligned(workspace, 256)) return W4A16_ERR_BAD_PLAN;
+  a.rows_form = p.rows_form;
+  a.cols = p.cols;
+  a.tiles = p.tiles;
+  a.splits = p.splits;
+  a.chunk = p.chunk;
+  a.part = static_cast<float*>(workspace);
+  return (int)launch_kv4_attention(a, stream_of(stream));
+}
+
+int w4a16_kv4_copy_pages(int32_t* pool, int64_t layers, int64_t pages, int64_t page_words,
+                         const int32_t* src, const int32_t* dst, int64_t n, void* stream) {
+  if (int e = pool_check(pool, layers, pages, page_words)) return e;
+  if (n < 0 || n > kMaxList) return W4A16_ERR_BAD_SHAPE;
+  if (n == 0 || layers == 0 || pages == 0) return W4A16_OK;
+  if (!src || !dst) return W4A16_ERR_NULL_POINTER;
+  return (int)launch_kv4_copy(pool, layers, pages, page_words, src, dst, n, stream_of(stream));
+}
+
+int w4a16_kv4_extend(const w4a16_kv4_book* book, const int32_t* seqs, const int32_t* counts,
+                     int64_t n, int32_t* status, void* stream) {
+  if (!book) return W4A16_ERR_NULL_POINTER;
+  if (int e = book_check(*book)) return e;
+  if (n < 0 || n > kMaxList) return W4A16_ERR_BAD_SHAPE;
+  if (n == 0) return W4A16_OK;
+  if (!seqs || !counts || !status) return W4A16_ERR_NULL_POINTER;
+  return (int)launch_kv4_extend(*book, seqs, counts, n, status, stream_of(stream));
+}
+
+size_t w4a16_kv4_fork_workspace_bytes(int64_t n) { return n > 0 ? (size_t)n * 8 : 0; }
+
+int w4a16_kv4_fork(int32_t* pool, int64_t layers, int64_t page_words, const w4a16_kv4_book* book,
+                   const int32_t* parents, const int32_t* children, int64_t n, int32_t* status,
+                   void* workspace, size_t workspace_bytes, void* stream) {
+  if (!book) return W4A16_ERR_NULL_POINTER;
+  if (int e = book_check(*book)) return e;
+  if (int e = pool_check(pool, layers, book->pages, page_words)) return e;
+  if (n < 0 || n > kMaxList) return W4A16_ERR_BAD_SHAPE;
+  if (n == 0) return W4A16_OK;
+  if (!parents || !children || !status) return W4A16_ERR_NULL_POINTER;
+  if (!workspace || workspace_bytes < w4a16_kv4_fork_workspace_bytes(n)) return W4A16_ERR_WORKSPACE;
+  return (int)launch_kv4_fork(pool, layers, page_words, *book, parents, children, n, status,
+                              static_cast<int32_t*>(workspace), stream_of(stream));
+}
+
+int w4a16_kv4_free(const w4a16_kv4_book* book, const int32_t* seqs, int64_t n, void* stream) {
+  if (!book) return W4A16_ERR_NULL_POINTER;
+  if (int e = book_check(*book)) return e;
+  if (n < 0 || n > kMaxList) return W4A16_ERR_BAD_SHAPE;
+  if (n == 0) return W4A16_OK;
+  if (!seqs) return W4A16_ERR_NULL_POINTER;
+  return (int)launch_kv4_free(*book, seqs, n, stream_of(stream));
+}
+
+size_t w4a16_kv4_compact_workspace_bytes(int64_t pages) {
+  return pages > 0 ? (size_t)(pages + 2 * (pages / 2 + 1) + 1) * 4 : 4;
+}
+
+int w4a16_kv4_compact(int32_t* pool, int64_t layers, int64_t page_words,
+                      const w4a16_kv4_book* book, int32_t* new_table, int32_t* new_refs,
+                      int32_t* live, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!book) return W4A16_ERR_NULL_POINTER;
+  if (int e = book_check(*book)) return e;
+  if (int e = pool_check(pool, layers, book->pages, page_words)) return e;
+  if (book->pages == 0) return W4A16_ERR_BAD_SHAPE;
+  if (!new_refs || !live || (book->rows && book->max_pages && !new_table))
+    return W4A16_ERR_NULL_POINTER;
+  if (new_refs == book->refs || new_table == book->table) return W4A16_ERR_BAD_PLAN;
+  if (!workspace || workspace_bytes < w4a16_kv4_compact_workspace_bytes(book->pages))
+    return W4A16_ERR_WORKSPACE;
+  return (int)launch_kv4_compact(pool, layers, page_words, *book, new_table, new_refs, live,
+                                 static_cast<int32_t*>(workspace), stream_of(stream));
+}
+
+}  // extern "C"

@@ -1,0 +1,557 @@
+// Attention over the 4-bit paged cache (format: kv4_device.h).
+//
+// For a query row r (one query token and head) and a stored token t with groups g:
+//   q . k_t       = sum_g  s_tg (q_g . code_tg - 8 Q_g) + c_tg Q_g,  Q_g = sum of q_g
+//   sum_t p_t v_t = sum_t (p_t s_tg) (code_tg - 8) + sum_t p_t c_tg
+// so the matrix cores multiply the codes themselves.  For keys a masked code word is
+// a pair of subnormal halves, code * 2^-24 (16 code * 2^-24 in its odd pairs, taken
+// out of the queries), which the matrix cores multiply exactly: five bitwise
+// instructions a word of eight codes, no conversion.  Queries are scaled by a power
+// of two into the top of fp16's range (exact), the -8 is the products' initial
+// value.  The sum of subnormal products is kept on a grid of 2^-24 of (the largest
+// query value of the step * 2^-14), that is 2^-14 of a code step times a query value:
+// a score is off by at most 2^-19 of what its terms could make it, far below the
+// rounding of the weights.  (Values do not go this way: there the same grid, which
+// rounds down, moved results of one-token weights by 5e-5 of a value's range.)  For
+// values a masked word with an exponent or-ed in is 1024 + code or 64 + code, and one
+// packed subtraction makes it code - 8, exactly: nine instructions a word.
+//
+// The weights p s of the values are rounded to fp16 (to nearest), the only rounding
+// below 32 bits; it acts on code - 8, the centres' sum stays in fp32.  They are
+// scaled by 2^(7 - E), E the exponent of the largest scale met so far: fp16 then
+// holds every weight down to 2^-29 of the largest to its full precision.  Scores,
+// maxima, denominators and all sums are fp32.
+//
+// A wave has 16 * C query rows and takes 32 tokens at a time: tokens are the rows
+// of the first product (two tiles of 16), so a lane holds the scores of one query
+// row and eight consecutive tokens, exactly the second product's operand.  The
+// running maximum moves only when a score exceeds it by 2^8 (or a value scale the
+// range above): then the sums are rescaled, else they are left alone, and the
+// branch is the wave's.
+//
+// Rows whose tokens are all hidden keep a denominator of 0 and become zeros.
+// Hidden tokens, and what lies behind the last one in a page, may hold anything:
+// scores and weights are selected, not multiplied, away.
+#pragma once
+
+#include "kv4_device.h"
+#include "kv4_launch.h"
+
+namespace w4a16 {
+
+constexpr int kAttnThreads = 256;
+constexpr float kNoScore = -1e30f;   // running maximum (in powers of two) before any score
+
+struct AttnArgs {
+  const uint16_t* q;
+  int64_t q_token, q_head;
+  uint16_t* out;
+  float *lse, *part;
+  const uint32_t* pool;
+  const int32_t *table, *lens, *starts, *seqs;
+  int table_rows, max_pages, pages, page_shift;
+  int heads, q_heads, per_kv, batch, tokens;
+  int tiles, splits, chunk, window;
+  float scale_log2;   // scale * log2(e)
+  bool causal, bf16, vec;
+};
+
+// What a row tile (rows r0 .. r0 + rows - 1 of sequence b and one kv head; row r is
+// query r / per_kv, head r % per_kv) reads.
+struct AttnSpan {
+  int row, n, q0, nq;    // table row, stored tokens, first query, queries
+  int lo, hi;            // tokens [lo, hi) that any of the rows sees
+  int first, active;     // first block of 32, splits that have any
+};
+__device__ __forceinline__ AttnSpan attn_span(const AttnArgs& a, int b, int r0, int rows) {
+  AttnSpan s;
+  s.row = a.seqs ? a.seqs[b] : b;
+  s.n = (uint32_t)s.row < (uint32_t)a.table_rows ? a.lens[s.row] : 0;
+  // (64 bits: max_pages pages may hold more than 2^31 tokens)
+  s.n = (int)min((int64_t)max(s.n, 0), min((int64_t)a.max_pages << a.page_shift, (int64_t)0x7fffffc0));
+  s.q0 = a.starts ? a.starts[b] : b;
+  s.nq = a.starts ? a.starts[b + 1] - s.q0 : 1;
+  if (s.q0 < 0 || s.q0 > a.tokens) s.nq = 0;
+  s.nq = max(0, min(s.nq, a.tokens - s.q0));
+  const int i0 = r0 / a.per_kv, i1 = min((r0 + rows - 1) / a.per_kv, s.nq - 1);
+  s.hi = a.causal ? max(0, s.n - s.nq + i1 + 1) : s.n;
+  s.lo = a.window > 0 ? min(max(0, s.n - s.nq + i0 - a.window + 1), s.hi) : 0;
+  if (i0 >= s.nq) s.hi = s.lo = 0;
+  s.first = s.lo >> 5;
+  const int blocks = s.hi > s.lo ? ((s.hi + 31) >> 5) - s.first : 0;
+  s.active = min(a.splits, (blocks + a.chunk - 1) / a.chunk);
+  return s;
+}
+
+// Combining two halves / four rows of a wave: every lane gets op over the lanes
+// that share its l % 16.
+template <class F>
+__device__ __forceinline__ float over_rows(float v, F op) {
+  float a = v, b = v;
+  permlane32_swap(a, b);
+  v = op(a, b);
+  a = v;
+  b = v;
+  permlane16_swap(a, b);
+  return op(a, b);
+}
+__device__ __forceinline__ float max_rows(float v) {
+  return over_rows(v, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float sum_rows(float v) {
+  return over_rows(v, [](float a, float b) { return a + b; });
+}
+
+// Eight codes as halves: code * 2^-24 at 0, 1, 4, 5, 16 * code * 2^-24 at 2, 3, 6, 7.
+__device__ __forceinline__ f16x8 code_halves(uint32_t w) {
+  const uint32_t t = w >> 8;
+  const u32x4 u = {w & 0x000F000Fu, w & 0x00F000F0u, t & 0x000F000Fu, t & 0x00F000F0u};
+  return __builtin_bit_cast(f16x8, u);
+}
+// Eight codes less 8.  `mg`: the two exponents (make_magic).
+__device__ __forceinline__ f16x8 value_halves(uint32_t w, const MagicRegs& mg) {
+  const uint32_t t = w >> 8;
+  const f16x2 a = {(f16)1032.0f, (f16)1032.0f}, b = {(f16)72.0f, (f16)72.0f};
+  const u32x4 u = {as_u32(as_h2(and_or(w, 0x000F000Fu, mg.m1024)) - a),
+                   as_u32(as_h2(and_or(w, 0x00F000F0u, mg.m64)) - b),
+                   as_u32(as_h2(and_or(t, 0x000F000Fu, mg.m1024)) - a),
+                   as_u32(as_h2(and_or(t, 0x00F000F0u, mg.m64)) - b)};
+  return __builtin_bit_cast(f16x8, u);
+}
+__device__ __forceinline__ float lo_f32(uint32_t w) { return (float)as_h((uint16_t)w); }
+__device__ __forceinline__ float hi_f32(uint32_t w) { return (float)as_h((uint16_t)(w >> 16)); }
+
+// One lane's words of 32 tokens: keys and values, with the group words of the
+// eight tokens that its scores belong to.
+template <int D, int NG>
+struct KvBlock {
+  uint32_t k[2][D / 32], v[D / 16], kg[NG][8], vg[NG][8];
+};
+
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t* dst, const uint32_t* p) {
+  if constexpr (N == 2) {
+    const u32x2 v = *reinterpret_cast<const u32x2*>(p);
+    dst[0] = v.x;
+    dst[1] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const u32x4 v = *reinterpret_cast<const u32x4*>(p + i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) dst[i + j] = v[j];
+    }
+  }
+}
+
+template <int D, int NG>
+__device__ __forceinline__ void load_block(KvBlock<D, NG>& x, const uint32_t* blk, int P, int t0,
+                                           int lane) {
+  const int c = lane & 15, g = lane >> 4;
+  const uint32_t* codes = blk + t0 * (D / 8);
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    load_words<D / 32>(x.k[j], codes + (8 * (c >> 2) + 4 * j + (c & 3)) * (D / 8) + g * (D / 32));
+#pragma unroll
+  for (int n = 0; n < NG; ++n)
+    load_words<8>(x.kg[n], blk + P * (D / 8) + n * P + t0 + 8 * g);
+#pragma unroll
+  for (int h = 0; h < D / 64; ++h)
+    load_words<4>(x.v + 4 * h, codes + P * (D / 8 + NG) + g * D + 64 * h + 4 * c);
+#pragma unroll
+  for (int n = 0; n < NG; ++n)
+    load_words<8>(x.vg[n], blk + P * (D / 4 + NG) + n * P + t0 + 8 * g);
+}
+
+template <int D, int NG, int C>
+struct AttnWave {
+  static constexpr int kSteps = D / 32, kTiles = D / 16;
+  f16x8 q[C][kSteps];
+  float Q[C][NG];              // sums of the scaled queries, 2^-24
+  float fac[C];                // score in powers of two = x * fac
+  int see_lo[C], see_hi[C];    // tokens that the lane's row sees
+  f32x4 acc[C][kTiles];
+  float m[C], l[C], csum[C][NG];
+  int E;
+  MagicRegs mg;
+
+  __device__ __forceinline__ void start() {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) acc[c][i] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int n = 0; n < NG; ++n) csum[c][n] = 0.0f;
+      m[c] = kNoScore;
+      l[c] = 0.0f;
+    }
+    E = -24;
+    mg = make_magic();
+  }
+
+  // Row `r` of the lane; rows past the tile's queries see nothing.
+  __device__ __forceinline__ void load_row(const AttnArgs& a, const AttnSpan& s, int h, int r,
+                                           int c, int lane) {
+    const int i = r / a.per_kv, hh = r - i * a.per_kv, g = lane >> 4;
+    const bool there = i < s.nq;
+    const int pos = s.n - s.nq + i;
+    see_hi[c] = there ? (a.causal ? min(max(pos + 1, 0), s.n) : s.n) : 0;
+    see_lo[c] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+    const uint16_t* src = a.q + (int64_t)(s.q0 + (there ? i : 0)) * a.q_token +
+                          (int64_t)(h * a.per_kv + (there ? hh : 0)) * a.q_head;
+    float x[kSteps][8], most = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      const u32x4 w = there ? load8(src + 32 * k + 8 * g, a.vec) : u32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint16_t u = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
+        x[k][j] = a.bf16 ? to_f32<true>(u) : to_f32<false>(u);
+        most = fmaxf(most, fabsf(x[k][j]));
+      }
+    }
+    most = max_rows(most);
+    // 2^e brings the largest value into [2^14, 2^15)
+    int e = 0;
+    if (most > 0.0f && most < __builtin_inff()) e = 15 - (__builtin_amdgcn_frexp_expf(most));
+#pragma unroll
+    for (int n = 0; n < NG; ++n) Q[c][n] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float y = ldexpf(x[k][j], e);
+        Q[c][k / (kSteps / NG)] += y;
+        q[c][k][j] = (f16)(j & 2 ? y * 0.0625f : y);
+      }
+#pragma unroll
+    for (int n = 0; n < NG; ++n) Q[c][n] = sum_rows(Q[c][n]) * 0x1p-24f;
+    fac[c] = ldexpf(a.scale_log2, 24 - e);
+  }
+
+  // 32 tokens from t on.  kMask: some of them are hidden from some row, or lie at
+  // or beyond n.
+  template <bool kMask>
+  __device__ __forceinline__ void step(const KvBlock<D, NG>& x, int t, int lane) {
+    const int g = lane >> 4, mine = t + 8 * g;
+    float sc[C][8];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      f32x4 s[C][NG];
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+          const float z = -8.0f * Q[c][n];
+          s[c][n] = f32x4{z, z, z, z};
+        }
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) {
+        const f16x8 w = code_halves(x.k[j][k]);
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+          s[c][k / (kSteps / NG)] =
+              __builtin_amdgcn_mfma_f32_16x16x32_f16(w, q[c][k], s[c][k / (kSteps / NG)], 0, 0, 0);
+      }
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float v = 0.0f;
+#pragma unroll
+          for (int n = 0; n < NG; ++n) {
+            const float u = hi_f32(x.kg[n][4 * j + r]) * Q[c][n];
+            v = fmaf(lo_f32(x.kg[n][4 * j + r]), s[c][n][r], n ? v + u : u);
+          }
+          if constexpr (kMask) {
+            const int tt = mine + 4 * j + r;
+            v = tt >= see_lo[c] && tt < see_hi[c] ? v : -__builtin_inff();
+          }
+          sc[c][4 * j + r] = v;
+        }
+    }
+    float big = 0.0f, sv[NG][8];
+    const float f = ldexpf(1.0f, 7 - E);
+#pragma unroll
+    for (int n = 0; n < NG; ++n)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float s = fmaf(lo_f32(x.vg[n][i]), f, 0.0f);
+        // what no row sees may hold anything
+        if constexpr (kMask) s = mine + i >= any_lo && mine + i < any_hi ? s : 0.0f;
+        sv[n][i] = s;
+        big = fmaxf(big, s);
+      }
+    float top[C];
+    bool move = !(big <= 128.0f);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      top[c] = fmaxf(fmaxf(fmaxf(sc[c][0], sc[c][1]), fmaxf(sc[c][2], sc[c][3])),
+                     fmaxf(fmaxf(sc[c][4], sc[c][5]), fmaxf(sc[c][6], sc[c][7])));
+      move |= top[c] * fac[c] > m[c] + 8.0f;
+    }
+    if (__ballot(move)) {
+      // (scales times 2^(7 - E); an infinite one spoils the rows that see it, and
+      // must not move the others' range)
+      float fine = 0.0f;
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          fine = fmaxf(fine, sv[n][i] < __builtin_inff() ? sv[n][i] : 0.0f);
+      const float most = ldexpf(max_rows(fine), E - 7);
+      const int E1 = max(E, __builtin_amdgcn_readfirstlane(most > 0.0f ? __builtin_amdgcn_frexp_expf(most) : -24));
+      const float down = ldexpf(1.0f, E - E1);
+      E = E1;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const float m1 = fmaxf(m[c], max_rows(top[c]) * fac[c]);
+        const float alpha = exp2f(m[c] - m1), all = alpha * down;
+        m[c] = m1;
+        l[c] *= alpha;
+#pragma unroll
+        for (int n = 0; n < NG; ++n) csum[c][n] *= alpha;
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) acc[c][i] *= all;
+      }
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sv[n][i] *= down;
+    }
+    f16x8 w[C][NG];
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(sc[c][i], fac[c], -m[c]));
+        l[c] += p;
+        const bool hidden = kMask && (mine + i < see_lo[c] || mine + i >= see_hi[c]);
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+          const float z = p * sv[n][i];
+          w[c][n][i] = (f16)(hidden ? 0.0f : z);
+          const float u = fmaf(p, hi_f32(x.vg[n][i]), csum[c][n]);
+          csum[c][n] = hidden ? csum[c][n] : u;
+        }
+      }
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+      const f16x8 v = value_halves(x.v[i], mg);
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        acc[c][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[c][i / (kTiles / NG)], acc[c][i],
+                                                           0, 0, 0);
+    }
+  }
+
+  // Blocks first, first + stride, ... below end.  Every one of the wave's rows sees
+  // the tokens [all_lo, all_hi), none sees others than [any_lo, any_hi).
+  int all_lo, all_hi, any_lo, any_hi;
+  __device__ __forceinline__ void run(const AttnArgs& a, const AttnSpan& s, int h, int first,
+                                      int end, int stride, int lane) {
+    const int P = 1 << a.page_shift, words = P * (D / 4 + 2 * NG);
+    const int32_t* pages = a.table + (int64_t)s.row * a.max_pages;
+    for (int kb = first; kb < end; kb += stride) {
+      const int t = kb << 5;
+      const int page = __builtin_amdgcn_readfirstlane(pages[t >> a.page_shift]);
+      if ((uint32_t)page >= (uint32_t)a.pages) continue;   // a missing page: its tokens are hidden
+      KvBlock<D, NG> x;
+      load_block(x, a.pool + ((int64_t)page * a.heads + h) * words, P, t & (P - 1), lane);
+      if (t < all_lo || t + 32 > all_hi)
+        step<true>(x, t, lane);
+      else
+        step<false>(x, t, lane);
+    }
+  }
+
+  // Sums over all the wave's tokens; then value d = 16 i + 4 (lane / 16) + j of the
+  // lane's row, not yet divided by l.
+  __device__ __forceinline__ void finish() {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      l[c] = sum_rows(l[c]);
+#pragma unroll
+      for (int n = 0; n < NG; ++n) csum[c][n] = sum_rows(csum[c][n]);
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          acc[c][i][j] = ldexpf(acc[c][i][j], E - 7) + csum[c][i / (kTiles / NG)];
+    }
+  }
+};
+
+// Place of a query row's partial result: values [splits][tokens * q_heads][D], then
+// (maximum, denominator) [splits][tokens * q_heads][2].
+__device__ __forceinline__ float* part_values(const AttnArgs& a, int split, int64_t qrow, int D) {
+  return a.part + ((int64_t)split * a.tokens * a.q_heads + qrow) * D;
+}
+__device__ __forceinline__ float* part_ml(const AttnArgs& a, int split, int64_t qrow, int D) {
+  return a.part + (int64_t)a.splits * a.tokens * a.q_heads * D +
+         ((int64_t)split * a.tokens * a.q_heads + qrow) * 2;
+}
+
+__device__ __forceinline__ void store4(uint16_t* p, const float v[4], bool bf16) {
+  u32x2 r;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    r[i] = bf16 ? (uint32_t)from_f32<true>(v[2 * i]) | (uint32_t)from_f32<true>(v[2 * i + 1]) << 16
+                : (uint32_t)from_f32<false>(v[2 * i]) | (uint32_t)from_f32<false>(v[2 * i + 1]) << 16;
+  *reinterpret_cast<u32x2*>(p) = r;
+}
+
+__device__ __forceinline__ float lse_of(float m, float l) {
+  return l > 0.0f || l != l ? (m + log2f(l)) * 0.6931471805599453f : -__builtin_inff();
+}
+
+// kRows false: the four waves share 16 * C rows and take blocks in turn; true: each
+// has 16 * C rows of its own.  Grid: kv head fastest (an XCD then keeps to few heads
+// and finds their codes in its L2), then split, sequence, and the row tiles from the
+// last, which sees the most tokens, to the first.
+template <int D, int NG, int C, bool kRows>
+__global__ __launch_bounds__(kAttnThreads) void kv4_attention_kernel(const AttnArgs a) {
+  constexpr int kTiles = D / 16;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint32_t id = blockIdx.x;
+  const int h = id % a.heads;
+  id /= a.heads;
+  const int split = id % a.splits;
+  id /= a.splits;
+  const int b = id % a.batch, tile = a.tiles - 1 - (int)(id / a.batch);
+  const int rows = kRows ? 64 * C : 16 * C;
+  const int r0 = tile * rows;
+  const AttnSpan s = attn_span(a, b, r0, rows);
+  const int R = s.nq * a.per_kv;
+  if (r0 >= R) return;
+  if (a.splits > 1 && split >= s.active) return;
+  const int w0 = kRows ? r0 + wave * 16 * C : r0;   // the wave's first row
+  if (kRows && w0 >= R) return;
+
+  AttnWave<D, NG, C> w;
+  w.start();
+#pragma unroll
+  for (int c = 0; c < C; ++c) w.load_row(a, s, h, w0 + 16 * c + (lane & 15), c, lane);
+  {
+    const int i0 = w0 / a.per_kv, i1 = min((w0 + 16 * C - 1) / a.per_kv, s.nq - 1);
+    // (rows past the last query see nothing, and need no mask to be ignored)
+    const int p0 = s.n - s.nq + i0, p1 = s.n - s.nq + i1;   // positions of first and last query
+    w.all_hi = a.causal ? min(max(p0 + 1, 0), s.n) : s.n;
+    w.any_hi = a.causal ? min(max(p1 + 1, 0), s.n) : s.n;
+    w.any_lo = a.window > 0 ? min(max(0, p0 - a.window + 1), w.any_hi) : 0;
+    w.all_lo = a.window > 0 ? max(0, p1 - a.window + 1) : 0;
+    // the split's blocks, as far as the wave's own rows see them
+    int first = s.first + split * a.chunk, end = (w.any_hi + 31) >> 5;
+    if (split + 1 < s.active) end = min(end, first + a.chunk);
+    if (kRows) first = max(first, w.any_lo >> 5);
+    w.run(a, s, h, kRows ? first : first + wave, end, kRows ? 1 : 4, lane);
+  }
+  w.finish();
+
+  const int col = lane & 15, g = lane >> 4;
+  if constexpr (kRows) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int r = w0 + 16 * c + col;
+      if (r >= R) continue;
+      const int i = r / a.per_kv;
+      const int64_t qrow = (int64_t)(s.q0 + i) * a.q_heads + h * a.per_kv + (r - i * a.per_kv);
+      if (a.splits > 1) {
+        float* dst = part_values(a, split, qrow, D);
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) *reinterpret_cast<f32x4*>(dst + 16 * t + 4 * g) = w.acc[c][t];
+        if (g == 0) {
+          float* ml = part_ml(a, split, qrow, D);
+          ml[0] = w.m[c];
+          ml[1] = w.l[c];
+        }
+      } else {
+        const bool any = w.l[c] > 0.0f || w.l[c] != w.l[c];
+        const float inv = any ? 1.0f / w.l[c] : 0.0f;
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+          float v[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = any ? w.acc[c][t][j] * inv : 0.0f;
+          store4(a.out + qrow * D + 16 * t + 4 * g, v, a.bf16);
+        }
+        if (a.lse && g == 0) a.lse[qrow] = lse_of(w.m[c], w.l[c]);
+      }
+    }
+  } else {
+    // (rows 4 floats apart beyond D: the four groups of lanes use different banks)
+    __shared__ float sum[4][16][D + 4];
+    __shared__ float ml[4][16][2];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      if (c) __syncthreads();
+      if (g == 0) {
+        ml[wave][col][0] = w.m[c];
+        ml[wave][col][1] = w.l[c];
+      }
+      __syncthreads();
+      const float m1 = fmaxf(fmaxf(ml[0][col][0], ml[1][col][0]), fmaxf(ml[2][col][0], ml[3][col][0]));
+      const float mine = exp2f(w.m[c] - m1);
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+        *reinterpret_cast<f32x4*>(&sum[wave][col][16 * t + 4 * g]) = w.acc[c][t] * mine;
+      __syncthreads();
+      // sixteen threads a row, four values at a time
+      const int rr = threadIdx.x >> 4, at = threadIdx.x & 15, r = r0 + 16 * c + rr;
+      if (r >= R) continue;
+      const float mm = fmaxf(fmaxf(ml[0][rr][0], ml[1][rr][0]), fmaxf(ml[2][rr][0], ml[3][rr][0]));
+      float l = 0.0f;
+#pragma unroll
+      for (int o = 0; o < 4; ++o) l += ml[o][rr][1] * exp2f(ml[o][rr][0] - mm);
+      const int i = r / a.per_kv;
+      const int64_t qrow = (int64_t)(s.q0 + i) * a.q_heads + h * a.per_kv + (r - i * a.per_kv);
+      const bool any = l > 0.0f || l != l;
+      const float inv = any ? 1.0f / l : 0.0f;
+#pragma unroll
+      for (int d = 0; d < D; d += 64) {
+        f32x4 v = *reinterpret_cast<f32x4*>(&sum[0][rr][d + 4 * at]);
+#pragma unroll
+        for (int o = 1; o < 4; ++o) v += *reinterpret_cast<f32x4*>(&sum[o][rr][d + 4 * at]);
+        if (a.splits > 1) {
+          *reinterpret_cast<f32x4*>(part_values(a, split, qrow, D) + d + 4 * at) = v;
+        } else {
+          float o[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[j] = any ? v[j] * inv : 0.0f;
+          store4(a.out + qrow * D + d + 4 * at, o, a.bf16);
+        }
+      }
+      if (at == 0) {
+        if (a.splits > 1) {
+          float* p = part_ml(a, split, qrow, D);
+          p[0] = mm;
+          p[1] = l;
+        } else if (a.lse) {
+          a.lse[qrow] = lse_of(mm, l);
+        }
+      }
+    }
+  }
+}
+
+// One form of the kernel for every head size and group count.
+template <int C, bool kRows>
+hipError_t launch_attention_form(const AttnArgs& a, int D, int NG, hipStream_t st) {
+  const dim3 grid((unsigned)a.heads * a.splits * a.batch * a.tiles), block(kAttnThreads);
+  switch (D * 8 + NG) {
+    case 64 * 8 + 1: kv4_attention_kernel<64, 1, C, kRows><<<grid, block, 0, st>>>(a); break;
+    case 64 * 8 + 2: kv4_attention_kernel<64, 2, C, kRows><<<grid, block, 0, st>>>(a); break;
+    case 128 * 8 + 1: kv4_attention_kernel<128, 1, C, kRows><<<grid, block, 0, st>>>(a); break;
+    case 128 * 8 + 2: kv4_attention_kernel<128, 2, C, kRows><<<grid, block, 0, st>>>(a); break;
+    case 128 * 8 + 4: kv4_attention_kernel<128, 4, C, kRows><<<grid, block, 0, st>>>(a); break;
+    case 256 * 8 + 1: kv4_attention_kernel<256, 1, C, kRows><<<grid, block, 0, st>>>(a); break;
+    case 256 * 8 + 2: kv4_attention_kernel<256, 2, C, kRows><<<grid, block, 0, st>>>(a); break;
+    default: kv4_attention_kernel<256, 4, C, kRows><<<grid, block, 0, st>>>(a); break;
+  }
+  return hipGetLastError();
+}
+hipError_t launch_attention_tokens1(const AttnArgs& a, int D, int NG, hipStream_t st);
+hipError_t launch_attention_tokens2(const AttnArgs& a, int D, int NG, hipStream_t st);
+hipError_t launch_attention_rows(const AttnArgs& a, int D, int NG, hipStream_t st);
+
+}  // namespace w4a16

@@ -1,0 +1,81 @@
+// The 4-bit paged key / value cache: its format, and what its kernels share.
+//
+// A pool is int32 [layers, pages, heads, words]; a block of `words` holds P tokens
+// of one page and head, in four parts:
+//   key codes    [P, D / 8]      key groups   [D / G, P]
+//   value codes  [P / 8, D]      value groups [D / G, P]
+// D values a head, G values a quantised group (along D, of one token).  A value is
+//   (code - 8) * scale + centre
+// with unsigned codes 0..15 and, per token and group, a word of two fp16 numbers,
+// the scale low and the centre high.  A code word holds eight codes, the i-th in
+// bits [4n, 4n + 4), n = i / 2 + 4 * (i % 2): masking a word with 0x000F000F and
+// 0x00F000F0, and both after a shift by eight, gives the codes as four pairs of
+// halves (0, 1), 16 (2, 3), (4, 5), 16 (6, 7).
+//   keys:   eight values 8o .. 8o + 7 of one token (octet o) in a word, octet o at
+//           word (D / 32) * (o % 4) + o / 4 of the token's row;
+//   values: one value d of eight tokens 8u .. 8u + 7 in a word, at word
+//           64 * (d / 64) + 4 * (d % 16) + d / 16 % 4 of row u.
+// These orders are the operands of v_mfma_f32_16x16x32_f16 as a lane holds them
+// (eight consecutive k, row or column lane % 16, lane / 16 choosing the octet of
+// k): one 16-byte load a lane brings the words of four steps, and an unpacked
+// word is an operand, so neither keys nor values pass through LDS.
+#pragma once
+
+#include "w4a16_device.h"
+
+namespace w4a16 {
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kKv4MinPage = 32;   // tokens: the attention kernel's step
+constexpr int kKv4MaxPage = 256;
+
+// Words of one block; the parts begin at 0, key_groups, values, value_groups.
+struct Kv4Layout {
+  int P, D, NG;
+  __host__ __device__ int key_groups() const { return P * D / 8; }
+  __host__ __device__ int values() const { return P * D / 8 + NG * P; }
+  __host__ __device__ int value_groups() const { return P * D / 4 + NG * P; }
+  __host__ __device__ int words() const { return P * D / 4 + 2 * NG * P; }
+};
+
+__device__ __forceinline__ int kv4_key_word(int octet, int D) {
+  return (D >> 5) * (octet & 3) + (octet >> 2);
+}
+__device__ __forceinline__ int kv4_value_word(int d) {
+  return (d & ~63) + 4 * (d & 15) + ((d >> 4) & 3);
+}
+__device__ __forceinline__ int kv4_shift(int i) { return 4 * ((i >> 1) + 4 * (i & 1)); }
+
+// Type of queries, keys, values and results.
+template <bool BF16>
+__device__ __forceinline__ float to_f32(uint16_t u) {
+  if constexpr (BF16) return __builtin_bit_cast(float, (uint32_t)u << 16);
+  return (float)as_h(u);
+}
+template <bool BF16>
+__device__ __forceinline__ uint16_t from_f32(float x) {
+  if constexpr (BF16) return __builtin_bit_cast(uint16_t, (__bf16)x);
+  return as_u16((f16)x);
+}
+
+// Eight consecutive values; `vec`: the address is 16-byte aligned.
+__device__ __forceinline__ u32x4 load8(const uint16_t* p, bool vec) {
+  if (vec) return *reinterpret_cast<const u32x4*>(p);
+  u32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = (uint32_t)p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+  return r;
+}
+
+// Block of a page: -1 where the table has none.  `row`, `at` are checked here, so
+// that no content of the tensors leads outside the pool.
+__device__ __forceinline__ int64_t kv4_page(const int32_t* __restrict__ table, int rows,
+                                            int max_pages, int pages, int row, int at) {
+  if ((uint32_t)row >= (uint32_t)rows || (uint32_t)at >= (uint32_t)max_pages) return -1;
+  const int p = table[(int64_t)row * max_pages + at];
+  return (uint32_t)p < (uint32_t)pages ? p : -1;
+}
+
+}  // namespace w4a16

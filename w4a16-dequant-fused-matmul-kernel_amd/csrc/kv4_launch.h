@@ -1,0 +1,54 @@
+// Host-side interface between the C-ABI layer (kv4_api.cpp) and the kernels of the
+// 4-bit paged cache.  Internal to libw4a16.so; not installed.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/w4a16.h"
+
+namespace w4a16 {
+
+// Queries and keys (and values) of `t`, normed and rotated; with `kv` the keys and
+// values are stored there, else the keys written to t.k_out.
+hipError_t launch_rope(const w4a16_rope& t, const w4a16_kv4* kv, const int32_t* rows,
+                       hipStream_t st);
+hipError_t launch_kv4_read(const w4a16_kv4& kv, const int32_t* positions, const int32_t* rows,
+                           int64_t tokens, void* k, void* v, bool bf16, hipStream_t st);
+
+// One attention call, planned (kv4_attention_plan).  A workgroup has four waves.
+//   rows_form: each wave has 16 * cols query rows of its own and all keys of the
+//              workgroup's range; else all waves have the same 16 * cols rows and
+//              take 32-token blocks in turn.
+// `chunk` blocks of 32 tokens to a split, the last split to the end; splits > 1
+// leave fp32 partials (unnormalised sums, then maximum and denominator) in `part`.
+struct Kv4Attn {
+  w4a16_kv4 kv;
+  w4a16_kv4_query q;
+  bool rows_form;
+  int cols, tiles, splits, chunk;
+  float* part;
+};
+struct Kv4Plan {
+  bool rows_form;
+  int cols, tiles, splits, chunk;
+  size_t workspace;
+};
+Kv4Plan kv4_attention_plan(const w4a16_kv4& kv, const w4a16_kv4_query& q);
+hipError_t launch_kv4_attention(const Kv4Attn& a, hipStream_t st);
+
+hipError_t launch_kv4_copy(int32_t* pool, int64_t layers, int64_t pages, int64_t page_words,
+                           const int32_t* src, const int32_t* dst, int64_t n, hipStream_t st);
+hipError_t launch_kv4_extend(const w4a16_kv4_book& b, const int32_t* seqs, const int32_t* counts,
+                             int64_t n, int32_t* status, hipStream_t st);
+hipError_t launch_kv4_fork(int32_t* pool, int64_t layers, int64_t page_words,
+                           const w4a16_kv4_book& b, const int32_t* parents,
+                           const int32_t* children, int64_t n, int32_t* status, int32_t* ws,
+                           hipStream_t st);
+hipError_t launch_kv4_free(const w4a16_kv4_book& b, const int32_t* seqs, int64_t n,
+                           hipStream_t st);
+hipError_t launch_kv4_compact(int32_t* pool, int64_t layers, int64_t page_words,
+                              const w4a16_kv4_book& b, int32_t* new_table, int32_t* new_refs,
+                              int32_t* live, int32_t* ws, hipStream_t st);
+
+}  // namespace w4a16

@@ -1,0 +1,405 @@
+// Pages of the 4-bit cache: copying, extending, forking, freeing, compacting.
+//
+// All bookkeeping stays on the device (page table, lengths, use counts), so a step
+// needs no wait for the host and can be replayed as a graph.  Free pages are taken
+// lowest first and lists are served in their order, by one workgroup that counts:
+// the result does not depend on timing.  The pages themselves are moved by as many
+// workgroups as keep the memory busy, every layer in one launch.
+#include "kv4_device.h"
+#include "kv4_launch.h"
+
+namespace w4a16 {
+namespace {
+
+constexpr int kPlan = 1024;   // threads of a counting workgroup
+constexpr int kMove = 256;
+
+// Exclusive sum of v over the workgroup's threads; *total gets the whole.
+__device__ __forceinline__ int block_scan(int v, int* total) {
+  __shared__ int part[kPlan / 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int s = v;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int o = __shfl_up(s, d);
+    if (lane >= d) s += o;
+  }
+  __syncthreads();   // the last call's sums have been read
+  if (lane == 63) part[wave] = s;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kPlan / 64; ++w) {
+    before += w < wave ? part[w] : 0;
+    all += part[w];
+  }
+  *total = all;
+  return before + s - v;
+}
+
+// Calls take(k, page) for the k-th page with refs == 0, k < want, lowest first;
+// returns how many there were, at most want.  All threads call it.
+template <class F>
+__device__ __forceinline__ int take_free(const int32_t* refs, int pages, int want, F take) {
+  int found = 0;
+  for (int p0 = 0; p0 < pages && found < want; p0 += 4 * kPlan) {
+    int free = 0;
+    bool is[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int p = p0 + 4 * (int)threadIdx.x + i;
+      is[i] = p < pages && refs[p] == 0;
+      free += is[i];
+    }
+    int total, k = found + block_scan(free, &total);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (is[i]) {
+        if (k < want) take(k, p0 + 4 * (int)threadIdx.x + i);
+        ++k;
+      }
+    found += total;
+  }
+  return min(found, want);
+}
+
+// Four words a thread; every page_words is a multiple of four (a block's words are).
+__device__ __forceinline__ void move_page(int32_t* pool, int64_t layer, int64_t pages,
+                                          int64_t page_words, int src, int dst, int piece,
+                                          int pieces) {
+  const u32x4* from =
+      reinterpret_cast<const u32x4*>(pool + (layer * pages + src) * page_words);
+  u32x4* to = reinterpret_cast<u32x4*>(pool + (layer * pages + dst) * page_words);
+  const int64_t n = page_words / 4;
+  for (int64_t i = (int64_t)piece * kMove + threadIdx.x; i < n; i += (int64_t)pieces * kMove)
+    to[i] = from[i];
+}
+
+// Pairs [0, n) (n on the device where count is given) over all layers; a workgroup
+// takes a piece of a page of a layer at a time.
+__global__ __launch_bounds__(kMove) void kv4_move_kernel(int32_t* pool, int64_t layers,
+                                                         int64_t pages, int64_t page_words,
+                                                         const int32_t* __restrict__ src,
+                                                         const int32_t* __restrict__ dst, int64_t n,
+                                                         const int32_t* count, int pieces) {
+  if (count) n = min(n, (int64_t)*count);
+  const int64_t all = n * layers * pieces;
+  for (int64_t u = blockIdx.x; u < all; u += gridDim.x) {
+    const int piece = (int)(u % pieces);
+    const int64_t pair = u / pieces % n, layer = u / pieces / n;
+    const int from = src[pair], to = dst[pair];
+    if ((uint64_t)(uint32_t)from >= (uint64_t)pages || (uint64_t)(uint32_t)to >= (uint64_t)pages ||
+        from < 0 || to < 0)
+      continue;
+    move_page(pool, layer, pages, page_words, from, to, piece, pieces);
+  }
+}
+
+struct Book {
+  int32_t *table, *lens, *refs;
+  int rows, max_pages, pages, page_shift;
+};
+
+__device__ __forceinline__ int pages_of(int64_t tokens, int shift) {
+  return (int)((tokens + (1 << shift) - 1) >> shift);
+}
+
+__device__ __forceinline__ void flag(int32_t* status, int bit) { atomicOr(status, bit); }
+
+// Rows seqs[i] grow by counts[i] tokens.  One workgroup: pages needed are summed in
+// the list's order, kPlan rows at a time, then the free pages are dealt out.  A
+// row that the pool cannot serve ends the dealing for the rows behind it as well.
+__global__ __launch_bounds__(kPlan) void kv4_extend_kernel(Book b, const int32_t* __restrict__ seqs,
+                                                           const int32_t* __restrict__ counts,
+                                                           int n, int32_t* status) {
+  __shared__ int first[kPlan], at[kPlan], row[kPlan];   // first page wanted, place in its row
+  for (int i0 = 0; i0 < n; i0 += kPlan) {
+    const int i = i0 + threadIdx.x;
+    int need = 0, r = -1, have = 0, add = 0;
+    if (i < n) {
+      r = seqs[i];
+      add = counts[i];
+      const bool ok = (uint32_t)r < (uint32_t)b.rows && add >= 0 && b.lens[r] >= 0;
+      if (!ok) {
+        flag(status, W4A16_KV4_BAD_ROW);
+        r = -1;
+      } else {
+        const int64_t len = b.lens[r];
+        have = pages_of(len, b.page_shift);
+        const int64_t want = pages_of(len + add, b.page_shift);
+        if (len + add > 0x7fffffff || want > b.max_pages) {
+          flag(status, W4A16_KV4_ROW_FULL);
+          r = -1;
+        } else {
+          need = (int)want - have;
+        }
+      }
+    }
+    int total;
+    const int from = block_scan(need, &total);
+    first[threadIdx.x] = from;
+    at[threadIdx.x] = have;
+    row[threadIdx.x] = r;
+    __syncthreads();
+    const int rows_here = min(kPlan, n - i0);
+    const int got = take_free(b.refs, b.pages, total, [&](int k, int page) {
+      // the row whose pages [first, first + need) hold k: the last with first <= k
+      int lo = 0, hi = rows_here - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (first[mid] <= k)
+          lo = mid;
+        else
+          hi = mid - 1;
+      }
+      b.table[(int64_t)row[lo] * b.max_pages + at[lo] + (k - first[lo])] = page;
+    });
+    __syncthreads();
+    if (r >= 0) {
+      if (from + need <= got) {
+        b.lens[r] += add;
+        for (int k = 0; k < need; ++k) {
+          int32_t* e = b.table + (int64_t)r * b.max_pages + have + k;
+          b.refs[*e] = 1;
+        }
+      } else {
+        flag(status, W4A16_KV4_NO_PAGES);
+        for (int k = 0; k < need; ++k) b.table[(int64_t)r * b.max_pages + have + k] = -1;
+      }
+    }
+    __threadfence_block();
+    __syncthreads();
+  }
+}
+
+// What children get: the page of the parent's partly filled last one (src, -1:
+// none) and the page that it is copied to (dst).  One workgroup.
+__global__ __launch_bounds__(kPlan) void kv4_fork_plan_kernel(Book b,
+                                                              const int32_t* __restrict__ parents,
+                                                              const int32_t* __restrict__ children,
+                                                              int n, int32_t* status, int32_t* src,
+                                                              int32_t* dst) {
+  __shared__ int fresh[kPlan];
+  for (int i0 = 0; i0 < n; i0 += kPlan) {
+    const int i = i0 + threadIdx.x;
+    int p = -1, c = -1, len = 0, need = 0;
+    if (i < n) {
+      p = parents[i];
+      c = children[i];
+      if ((uint32_t)p >= (uint32_t)b.rows || (uint32_t)c >= (uint32_t)b.rows || p == c ||
+          b.lens[c] != 0 || b.lens[p] < 0) {
+        flag(status, W4A16_KV4_BAD_ROW);
+        c = -1;
+      } else {
+        len = b.lens[p];
+        need = (len & ((1 << b.page_shift) - 1)) != 0;
+      }
+    }
+    int total;
+    const int from = block_scan(need, &total);
+    const int got = take_free(b.refs, b.pages, total, [&](int k, int page) { fresh[k] = page; });
+    __syncthreads();
+    const bool served = c >= 0 && from + need <= got;
+    if (c >= 0 && !served) flag(status, W4A16_KV4_NO_PAGES);
+    if (i < n) {
+      const int last = len >> b.page_shift;
+      src[i] = served && need && last < b.max_pages ? b.table[(int64_t)p * b.max_pages + last] : -1;
+      dst[i] = served ? (need ? fresh[from] : -1) : -2;   // -2: this child gets nothing
+      if (served && need) b.refs[fresh[from]] = 1;
+    }
+    __threadfence_block();
+    __syncthreads();
+  }
+}
+
+// Rows of the children (workgroups [0, n)) and the copies (the others).  No page
+// is both copied from and to: fresh ones were free.
+__global__ __launch_bounds__(kMove) void kv4_fork_kernel(Book b, int32_t* pool, int64_t layers,
+                                                         int64_t page_words,
+                                                         const int32_t* __restrict__ parents,
+                                                         const int32_t* __restrict__ children,
+                                                         int n, const int32_t* __restrict__ src,
+                                                         const int32_t* __restrict__ dst,
+                                                         int pieces) {
+  if ((int)blockIdx.x < n) {
+    const int i = blockIdx.x, to = dst[i];
+    if (to == -2) return;
+    const int p = parents[i], c = children[i], len = b.lens[p];
+    const int whole = min(len >> b.page_shift, b.max_pages);
+    const int32_t* from = b.table + (int64_t)p * b.max_pages;
+    int32_t* row = b.table + (int64_t)c * b.max_pages;
+    for (int k = threadIdx.x; k < b.max_pages; k += kMove) {
+      int page = -1;
+      if (k < whole) {
+        page = from[k];
+        if ((uint32_t)page < (uint32_t)b.pages) atomicAdd(b.refs + page, 1);
+      } else if (k == whole && to >= 0) {
+        page = to;
+      }
+      row[k] = page;
+    }
+    if (threadIdx.x == 0) b.lens[c] = len;
+    return;
+  }
+  const int64_t all = (int64_t)n * layers * pieces;
+  for (int64_t u = (int64_t)blockIdx.x - n; u < all; u += (int64_t)gridDim.x - n) {
+    const int piece = (int)(u % pieces);
+    const int64_t pair = u / pieces % n, layer = u / pieces / n;
+    const int from = src[pair], to = dst[pair];
+    if ((uint32_t)from >= (uint32_t)b.pages || (uint32_t)to >= (uint32_t)b.pages) continue;
+    move_page(pool, layer, b.pages, page_words, from, to, piece, pieces);
+  }
+}
+
+// A row's entries are taken out one by one: a row that is named twice gives its
+// pages back once.
+__global__ __launch_bounds__(kMove) void kv4_free_kernel(Book b, const int32_t* __restrict__ seqs) {
+  const int r = seqs[blockIdx.x];
+  if ((uint32_t)r >= (uint32_t)b.rows) return;
+  for (int k = threadIdx.x; k < b.max_pages; k += kMove) {
+    int32_t* e = b.table + (int64_t)r * b.max_pages + k;
+    if (*e == -1) continue;
+    const int page = atomicExch(e, -1);
+    if ((uint32_t)page < (uint32_t)b.pages) atomicSub(b.refs + page, 1);
+  }
+  if (threadIdx.x == 0) b.lens[r] = 0;
+}
+
+// to[p]: where page p lies afterwards; src, dst: the moves, counts[0] of them.
+// One workgroup: the live pages are counted, then movers and holes ranked together.
+__global__ __launch_bounds__(kPlan) void kv4_compact_plan_kernel(const int32_t* __restrict__ refs,
+                                                                 int pages, int32_t* new_refs,
+                                                                 int32_t* live_out, int32_t* to,
+                                                                 int32_t* src, int32_t* dst,
+                                                                 int32_t* counts) {
+  int mine = 0, total;
+  for (int p = threadIdx.x; p < pages; p += kPlan) mine += refs[p] > 0;
+  block_scan(mine, &total);
+  const int live = total;
+  int movers = 0, holes = 0;
+  for (int p0 = 0; p0 < pages; p0 += kPlan) {
+    const int p = p0 + threadIdx.x;
+    const bool used = p < pages && refs[p] > 0;
+    const bool moves = used && p >= live, hole = p < live && p < pages && !used;
+    // a span of pages has movers or holes, or, where live falls inside it, both
+    int tm, th;
+    const int km = movers + block_scan(moves, &tm);
+    const int kh = holes + block_scan(hole, &th);
+    if (moves) src[km] = p;
+    if (hole) dst[kh] = p;
+    if (p < pages) to[p] = p;
+    movers += tm;
+    holes += th;
+  }
+  __threadfence_block();
+  __syncthreads();
+  for (int p = threadIdx.x; p < pages; p += kPlan) new_refs[p] = p < live ? max(refs[p], 0) : 0;
+  __threadfence_block();
+  __syncthreads();
+  for (int k = threadIdx.x; k < movers; k += kPlan) {
+    to[src[k]] = dst[k];
+    new_refs[dst[k]] = refs[src[k]];
+  }
+  if (threadIdx.x == 0) {
+    counts[0] = movers;
+    *live_out = live;
+  }
+}
+
+__global__ __launch_bounds__(kMove) void kv4_compact_kernel(
+    int32_t* pool, int64_t layers, int64_t pages, int64_t page_words,
+    const int32_t* __restrict__ src, const int32_t* __restrict__ dst, const int32_t* counts,
+    int pieces, const int32_t* __restrict__ table, int32_t* __restrict__ new_table,
+    int64_t entries, const int32_t* __restrict__ to, int table_blocks) {
+  if ((int)blockIdx.x < table_blocks) {
+    for (int64_t i = (int64_t)blockIdx.x * kMove + threadIdx.x; i < entries;
+         i += (int64_t)table_blocks * kMove) {
+      const int p = table[i];
+      new_table[i] = (uint64_t)(uint32_t)p < (uint64_t)pages && p >= 0 ? to[p] : -1;
+    }
+    return;
+  }
+  const int64_t n = counts[0], all = n * layers * pieces;
+  for (int64_t u = (int64_t)blockIdx.x - table_blocks; u < all;
+       u += (int64_t)gridDim.x - table_blocks) {
+    const int piece = (int)(u % pieces);
+    const int64_t pair = u / pieces % n, layer = u / pieces / n;
+    move_page(pool, layer, pages, page_words, src[pair], dst[pair], piece, pieces);
+  }
+}
+
+Book book_of(const w4a16_kv4_book& b) {
+  return Book{b.table, b.lens, b.refs, (int)b.rows, (int)b.max_pages, (int)b.pages,
+              __builtin_ctz((unsigned)b.page_size)};
+}
+
+// A piece is about 16 KB: few enough to a page that its address is worked out
+// seldom, small enough that a few pages fill the chip.
+int pieces_of(int64_t page_words) {
+  const int64_t p = (page_words + 4095) / 4096;
+  return (int)(p < 1 ? 1 : p);
+}
+constexpr int64_t kMoveBlocks = 2048;   // eight workgroups a CU
+
+unsigned move_blocks(int64_t n, int64_t layers, int pieces) {
+  const int64_t all = n * layers * pieces;
+  return (unsigned)(all < kMoveBlocks ? all : kMoveBlocks);
+}
+
+}  // namespace
+
+hipError_t launch_kv4_copy(int32_t* pool, int64_t layers, int64_t pages, int64_t page_words,
+                           const int32_t* src, const int32_t* dst, int64_t n, hipStream_t st) {
+  const int pieces = pieces_of(page_words);
+  kv4_move_kernel<<<move_blocks(n, layers, pieces), kMove, 0, st>>>(
+      pool, layers, pages, page_words, src, dst, n, nullptr, pieces);
+  return hipGetLastError();
+}
+
+hipError_t launch_kv4_extend(const w4a16_kv4_book& b, const int32_t* seqs, const int32_t* counts,
+                             int64_t n, int32_t* status, hipStream_t st) {
+  kv4_extend_kernel<<<1, kPlan, 0, st>>>(book_of(b), seqs, counts, (int)n, status);
+  return hipGetLastError();
+}
+
+hipError_t launch_kv4_fork(int32_t* pool, int64_t layers, int64_t page_words,
+                           const w4a16_kv4_book& b, const int32_t* parents,
+                           const int32_t* children, int64_t n, int32_t* status, int32_t* ws,
+                           hipStream_t st) {
+  int32_t *src = ws, *dst = ws + n;
+  kv4_fork_plan_kernel<<<1, kPlan, 0, st>>>(book_of(b), parents, children, (int)n, status, src,
+                                            dst);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const int pieces = pieces_of(page_words);
+  kv4_fork_kernel<<<(unsigned)n + move_blocks(n, layers, pieces), kMove, 0, st>>>(
+      book_of(b), pool, layers, page_words, parents, children, (int)n, src, dst, pieces);
+  return hipGetLastError();
+}
+
+hipError_t launch_kv4_free(const w4a16_kv4_book& b, const int32_t* seqs, int64_t n,
+                           hipStream_t st) {
+  kv4_free_kernel<<<(unsigned)n, kMove, 0, st>>>(book_of(b), seqs);
+  return hipGetLastError();
+}
+
+hipError_t launch_kv4_compact(int32_t* pool, int64_t layers, int64_t page_words,
+                              const w4a16_kv4_book& b, int32_t* new_table, int32_t* new_refs,
+                              int32_t* live, int32_t* ws, hipStream_t st) {
+  const int64_t half = b.pages / 2 + 1;
+  int32_t *to = ws, *src = ws + b.pages, *dst = src + half, *counts = dst + half;
+  kv4_compact_plan_kernel<<<1, kPlan, 0, st>>>(b.refs, (int)b.pages, new_refs, live, to, src, dst,
+                                               counts);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const int pieces = pieces_of(page_words);
+  const int64_t entries = b.rows * b.max_pages;
+  const int64_t tb = (entries + 1023) / 1024 + 1;
+  const int table_blocks = (int)(tb < 64 ? tb : 64);
+  kv4_compact_kernel<<<(unsigned)table_blocks + move_blocks(half, layers, pieces), kMove, 0, st>>>(
+      pool, layers, b.pages, page_words, src, dst, counts, pieces, b.table, new_table, entries, to,
+      table_blocks);
+  return hipGetLastError();
+}
+
+}  // namespace w4a16

@@ -21,8 +21,10 @@ BUILD_DIR = os.path.join(CSRC, "_build")
 LIB_PATH = os.path.join(PKG_DIR, "libw4a16.so")
 SOURCES = ["gemv.hip", "gemm_mfma.hip", "gemm_occ2.hip", "gemm_stream.hip", "gemm_skinny.hip",
            "gemm_wide_256.hip", "gemm_wide_128.hip", "gemm_wide_64.hip", "simt.hip", "quant.hip",
-           "capi.cpp"]
-HEADERS = ["w4a16_device.h", "w4a16_launch.h", "gemm_wide.h", "decode_table.inc"]
+           "kv4_append.hip", "kv4_attention.hip", "kv4_attn_tokens1.hip", "kv4_attn_tokens2.hip",
+           "kv4_attn_rows.hip", "kv4_pages.hip", "kv4_api.cpp", "capi.cpp"]
+HEADERS = ["w4a16_device.h", "w4a16_launch.h", "gemm_wide.h", "decode_table.inc",
+           "kv4_device.h", "kv4_launch.h", "kv4_attn.h"]
 PUBLIC_HEADER = os.path.join(os.path.dirname(ROOT_DIR), "include", "w4a16.h")
 ARCH = "gfx950"
 

@@ -67,6 +67,64 @@ class Plan(ctypes.Structure):
         return d
 
 
+class Rope(ctypes.Structure):
+    """Mirror of ``struct w4a16_rope``."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("q_token", ctypes.c_int64), ("q_head", ctypes.c_int64),
+        ("k_token", ctypes.c_int64), ("k_head", ctypes.c_int64),
+        ("v_token", ctypes.c_int64), ("v_head", ctypes.c_int64),
+        ("q_out", ctypes.c_void_p), ("k_out", ctypes.c_void_p),
+        ("cos", ctypes.c_void_p), ("sin", ctypes.c_void_p),
+        ("token_position", ctypes.c_void_p),
+        ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p),
+        ("tokens", ctypes.c_int64), ("positions", ctypes.c_int64),
+        ("q_heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("rot_dim", ctypes.c_int32),
+        ("eps", ctypes.c_float), ("flags", ctypes.c_int32),
+    ]
+
+
+class KV4(ctypes.Structure):
+    """Mirror of ``struct w4a16_kv4``."""
+
+    _fields_ = [
+        ("pool", ctypes.c_void_p), ("table", ctypes.c_void_p),
+        ("pages", ctypes.c_int64), ("rows", ctypes.c_int64), ("max_pages", ctypes.c_int64),
+        ("heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+        ("group_size", ctypes.c_int32), ("page_size", ctypes.c_int32),
+    ]
+
+
+class KV4Query(ctypes.Structure):
+    """Mirror of ``struct w4a16_kv4_query``."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("q_token", ctypes.c_int64), ("q_head", ctypes.c_int64),
+        ("out", ctypes.c_void_p), ("lse", ctypes.c_void_p), ("lens", ctypes.c_void_p),
+        ("q_starts", ctypes.c_void_p), ("seqs", ctypes.c_void_p),
+        ("tokens", ctypes.c_int64), ("batch", ctypes.c_int64),
+        ("max_q", ctypes.c_int64), ("max_context", ctypes.c_int64),
+        ("q_heads", ctypes.c_int32), ("window", ctypes.c_int32),
+        ("scale", ctypes.c_float), ("flags", ctypes.c_int32),
+    ]
+
+
+class KV4Book(ctypes.Structure):
+    """Mirror of ``struct w4a16_kv4_book``."""
+
+    _fields_ = [
+        ("table", ctypes.c_void_p), ("lens", ctypes.c_void_p), ("refs", ctypes.c_void_p),
+        ("rows", ctypes.c_int64), ("max_pages", ctypes.c_int64), ("pages", ctypes.c_int64),
+        ("page_size", ctypes.c_int32),
+    ]
+
+
+# flags of the 4-bit cache's calls, and the bits its page calls set in a status
+KV4_BF16, KV4_INTERLEAVED, KV4_CAUSAL = 1, 2, 4
+KV4_NO_PAGES, KV4_ROW_FULL, KV4_BAD_ROW = 1, 2, 4
+
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int32
@@ -109,6 +167,23 @@ SIGNATURES = {
     "w4a16_pack_int4": (_int, [_vp, _vp, _i64, _i64, _vp, _vp]),
     "w4a16_unpack_int4": (_int, [_vp, _vp, _i64, _i64, _vp]),
     "w4a16_dequantize_f16": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
+    "w4a16_kv4_words": (_i64, [_i32, _i32, _i32]),
+    "w4a16_qk_norm_rope": (_int, [ctypes.POINTER(Rope), _vp]),
+    "w4a16_kv4_append": (_int, [ctypes.POINTER(Rope), ctypes.POINTER(KV4), _vp, _vp]),
+    "w4a16_kv4_read": (_int, [ctypes.POINTER(KV4), _vp, _vp, _i64, _vp, _vp, _i32, _vp]),
+    "w4a16_kv4_attention_workspace_bytes": (
+        _sz, [ctypes.POINTER(KV4), ctypes.POINTER(KV4Query)]),
+    "w4a16_kv4_attention": (
+        _int, [ctypes.POINTER(KV4), ctypes.POINTER(KV4Query), _vp, _sz, _vp]),
+    "w4a16_kv4_copy_pages": (_int, [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp]),
+    "w4a16_kv4_extend": (_int, [ctypes.POINTER(KV4Book), _vp, _vp, _i64, _vp, _vp]),
+    "w4a16_kv4_fork_workspace_bytes": (_sz, [_i64]),
+    "w4a16_kv4_fork": (
+        _int, [_vp, _i64, _i64, ctypes.POINTER(KV4Book), _vp, _vp, _i64, _vp, _vp, _sz, _vp]),
+    "w4a16_kv4_free": (_int, [ctypes.POINTER(KV4Book), _vp, _i64, _vp]),
+    "w4a16_kv4_compact_workspace_bytes": (_sz, [_i64]),
+    "w4a16_kv4_compact": (
+        _int, [_vp, _i64, _i64, ctypes.POINTER(KV4Book), _vp, _vp, _vp, _vp, _sz, _vp]),
 }
 
 _LIB = None

@@ -1,0 +1,127 @@
+"""A 4-bit paged cache over all layers of a model, and an attention layer on it.
+
+``KV4Cache`` keeps the pool and its bookkeeping on the device and offers the page
+calls of :mod:`w4a16.kv4` on them.  ``W4A16Attention`` runs them together as a
+W4A16 decoder layer does: fused QKV projection, norm and rotation with the storing,
+attention over the cache, output projection.
+"""
+from __future__ import annotations
+
+import torch
+from torch import Tensor, nn
+
+from . import _lib
+from . import kv4
+from .linear import W4A16Linear
+
+__all__ = ["KV4Cache", "W4A16Attention"]
+
+
+class KV4Cache:
+    """Keys and values of ``sequences`` rows in 4 bits, in pages shared by ``layers``.
+
+    * ``pool``  int32 [layers, pages, heads, words]
+    * ``table`` int32 [sequences, max_pages], page ids in order, -1 where none
+    * ``lens``  int32 [sequences], tokens of a row
+    * ``refs``  int32 [pages], rows that hold a page
+    * ``status`` int32 [1], what went wrong so far (``NO_PAGES``, ``ROW_FULL``,
+      ``BAD_ROW``); ``check()`` waits for the device and raises
+
+    The calls take device tensors and wait for nothing, so a step made of them can
+    be captured into a HIP graph (``compact`` apart: it replaces two tensors).
+    """
+
+    NO_PAGES, ROW_FULL, BAD_ROW = _lib.KV4_NO_PAGES, _lib.KV4_ROW_FULL, _lib.KV4_BAD_ROW
+
+    def __init__(self, layers: int, pages: int, heads: int, head_dim: int, *, sequences: int,
+                 max_pages: int, page_size: int = 64, group_size: int = 64,
+                 device: torch.device | str = "cuda") -> None:
+        words = kv4.kv4_words(head_dim, group_size, page_size)
+        self.heads, self.head_dim = heads, head_dim
+        self.page_size, self.group_size = page_size, group_size
+        self.pool = torch.zeros((layers, pages, heads, words), dtype=torch.int32, device=device)
+        self.table = torch.full((sequences, max_pages), -1, dtype=torch.int32, device=device)
+        self.lens = torch.zeros(sequences, dtype=torch.int32, device=device)
+        self.refs = torch.zeros(pages, dtype=torch.int32, device=device)
+        self.status = torch.zeros(1, dtype=torch.int32, device=device)
+
+    def extend(self, seqs: Tensor, counts: Tensor) -> None:
+        """Pages for ``counts[i]`` new tokens of row ``seqs[i]``; ``lens`` grows."""
+        kv4.kv4_extend(self.table, self.lens, self.refs, seqs, counts, page_size=self.page_size,
+                       status=self.status)
+
+    def fork(self, parents: Tensor, children: Tensor) -> None:
+        """Empty rows ``children`` become copies of rows ``parents``."""
+        kv4.kv4_fork(self.pool, self.table, self.lens, self.refs, parents, children,
+                     page_size=self.page_size, status=self.status)
+
+    def free(self, seqs: Tensor) -> None:
+        """Empty rows ``seqs``."""
+        kv4.kv4_free(self.table, self.lens, self.refs, seqs)
+
+    def compact(self) -> Tensor:
+        """Move the pages in use to the front; int32 [1], how many they are."""
+        self.table, self.refs, live = kv4.kv4_compact(self.pool, self.table, self.refs)
+        return live
+
+    def copy_pages(self, src: Tensor, dst: Tensor) -> None:
+        """Page ``src[i]`` to ``dst[i]`` in every layer."""
+        kv4.kv4_copy_pages(self.pool, src, dst)
+
+    def check(self) -> None:
+        """Wait for the device; RuntimeError if a call could not be served."""
+        s = int(self.status.item())
+        if s:
+            what = [t for bit, t in ((self.NO_PAGES, "the pool had no free page"),
+                                     (self.ROW_FULL, "a row's table is full"),
+                                     (self.BAD_ROW, "a row that does not exist, a negative count "
+                                                    "or a child in use")) if s & bit]
+            raise RuntimeError("KV4Cache: " + "; ".join(what))
+
+    def append(self, layer: int, q: Tensor, k: Tensor, v: Tensor, cos: Tensor, sin: Tensor,
+               positions: Tensor, rows: Tensor | None = None, **norm) -> Tensor:
+        """``kv4_append`` into one layer; the rotated queries."""
+        return kv4.kv4_append(q, k, v, cos, sin, positions, self.pool[layer], self.table,
+                              rows=rows, group_size=self.group_size, **norm)
+
+    def attend(self, layer: int, q: Tensor, **how) -> Tensor:
+        """``kv4_attention`` over one layer."""
+        return kv4.kv4_attention(q, self.pool[layer], self.table, self.lens,
+                                 group_size=self.group_size, **how)
+
+
+class W4A16Attention(nn.Module):
+    """Self-attention of a W4A16 decoder layer over a ``KV4Cache``.
+
+    ``qkv`` and ``out`` are ``W4A16Linear``; with ``qk_norm`` every query and key
+    head is normed.  The caller extends the cache by the step's tokens first.
+    """
+
+    def __init__(self, hidden: int, q_heads: int, kv_heads: int, head_dim: int, layer: int = 0, *,
+                 group_size: int = 128, qk_norm: bool = True, bias: bool = False,
+                 eps: float = 1e-6, device: torch.device | str | None = None) -> None:
+        super().__init__()
+        if kv_heads < 1 or q_heads % kv_heads:
+            raise ValueError(f"W4A16Attention: {q_heads} query heads are not a multiple of "
+                             f"{kv_heads} key / value heads")
+        self.q_heads, self.kv_heads, self.head_dim = q_heads, kv_heads, head_dim
+        self.layer, self.eps = layer, eps
+        self.qkv = W4A16Linear(hidden, (q_heads + 2 * kv_heads) * head_dim, group_size, bias,
+                               device)
+        self.out = W4A16Linear(q_heads * head_dim, hidden, group_size, bias, device)
+        for name in ("q_norm", "k_norm"):
+            w = torch.ones(head_dim, dtype=torch.float16, device=device) if qk_norm else None
+            self.register_buffer(name, w)
+
+    def forward(self, x: Tensor, cache: KV4Cache, positions: Tensor, cos: Tensor, sin: Tensor, *,
+                rows: Tensor | None = None, interleaved: bool = False, **how) -> Tensor:
+        """x fp16 [tokens, hidden] at ``positions`` (int32) of cache rows ``rows``
+        (None: token i in row i); ``how`` goes to ``kv4_attention`` (q_starts, seqs,
+        max_q, max_context, window)."""
+        T, H = x.shape[0], self.q_heads + self.kv_heads
+        qkv = self.qkv(x).view(T, H + self.kv_heads, self.head_dim)
+        q = cache.append(self.layer, qkv[:, :self.q_heads], qkv[:, self.q_heads:H], qkv[:, H:],
+                         cos, sin, positions, rows, q_weight=self.q_norm, k_weight=self.k_norm,
+                         eps=self.eps, interleaved=interleaved)
+        y = cache.attend(self.layer, q, **how)
+        return self.out(y.view(T, self.q_heads * self.head_dim))

@@ -1,0 +1,422 @@
+"""A 4-bit paged key / value cache: storing, attending, and moving its pages.
+
+What an attention layer of a W4A16 model needs between its fused QKV projection
+and its output projection.  No counterpart in the reference (a GEMM alone).
+
+* ``qk_norm_rope``    per-head RMS norm and position rotation of queries and keys
+* ``kv4_append``      the same, keys and values stored in 4 bits in one launch
+* ``kv4_read``        stored tokens back as dense tensors
+* ``kv4_attention``   attention over the stored tokens: one new token a sequence,
+                      several, or prompts
+* ``kv4_extend`` / ``kv4_fork`` / ``kv4_free`` / ``kv4_compact`` /
+  ``kv4_copy_pages``  the pages
+
+``pool`` is int32 [pages, heads, words] (one layer) or [layers, pages, heads,
+words] for the calls that move pages; ``words = kv4_words(head_dim, group_size,
+page_size)``.  Every ``group_size`` values of one token's head share an fp16 scale
+and an fp16 centre, ``value = (code - 8) * scale + centre`` (layout:
+``include/w4a16.h``).  ``table`` int32 [rows, max_pages] holds a sequence's page
+ids in order, -1 where there is none; ``lens`` int32 [rows] its tokens; ``refs``
+int32 [pages] how many rows hold a page.
+
+Head sizes 64, 128 and 256; groups of D, D/2 or D/4 (at least 32); pages of 32,
+64, 128 or 256 tokens; queries, keys and values in fp16 or bf16 (the new tokens'
+``q``, ``k``, ``v`` may be slices of one fused projection: any token and head
+strides).  Bad arguments raise ``AssertionError``; everything runs in hand-written
+HIP kernels on the current stream, without waiting for the device, and can be
+captured into a HIP graph.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+from torch import Tensor
+
+from . import _lib
+from . import _runtime as rt
+
+__all__ = ["qk_norm_rope", "kv4_append", "kv4_read", "kv4_attention", "kv4_copy_pages",
+           "kv4_extend", "kv4_fork", "kv4_free", "kv4_compact", "kv4_words"]
+
+_TYPES = (torch.float16, torch.bfloat16)
+
+
+def kv4_words(head_dim: int, group_size: int, page_size: int) -> int:
+    """int32 words of one page and head (AssertionError for sizes the cache lacks)."""
+    n = int(rt.lib().w4a16_kv4_words(head_dim, group_size, page_size))
+    assert n > 0, (f"no 4-bit cache of head_dim={head_dim}, group_size={group_size}, "
+                   f"page_size={page_size}: head_dim is 64, 128 or 256, group_size head_dim / 1, 2 "
+                   "or 4 and at least 32, page_size 32, 64, 128 or 256")
+    return n
+
+
+def _int32(t: Tensor, name: str, shape: tuple, dev: torch.device) -> Tensor:
+    assert t.dtype == torch.int32, f"{name} must be int32, got {t.dtype}"
+    assert t.device == dev, f"{name} must be on {dev}, got {t.device}"
+    assert tuple(t.shape) == shape, f"{name} must be {list(shape)}, got {list(t.shape)}"
+    assert t.is_contiguous(), f"{name} must be contiguous"
+    return t
+
+
+def _heads3(t: Tensor, name: str, like: Tensor | None = None) -> Tensor:
+    assert t.is_cuda, f"{name} must be on a HIP device"
+    assert t.dim() == 3, f"{name} must be [tokens, heads, head_dim], got {list(t.shape)}"
+    assert t.dtype in _TYPES, f"{name} must be fp16 or bf16, got {t.dtype}"
+    assert t.shape[2] == 1 or t.stride(2) == 1, f"{name} must have unit stride inside a head"
+    if like is not None:
+        assert t.dtype == like.dtype and t.device == like.device, \
+            f"{name} must have the queries' type and device"
+        assert t.shape[0] == like.shape[0] and t.shape[2] == like.shape[2], \
+            f"{name} must have the queries' tokens and head size"
+    return t
+
+
+def _page_size(pool: Tensor, head_dim: int, group_size: int) -> int:
+    """Tokens of a page, from the pool's words."""
+    assert head_dim in (64, 128, 256), f"head_dim must be 64, 128 or 256, got {head_dim}"
+    assert group_size >= 32 and head_dim in (group_size, 2 * group_size, 4 * group_size), (
+        f"group_size={group_size} must be head_dim={head_dim}, a half or a quarter of it, and at "
+        "least 32")
+    P, rest = divmod(pool.shape[-1], head_dim // 4 + 2 * (head_dim // group_size))
+    assert rest == 0 and P in (32, 64, 128, 256), (
+        f"a pool of {pool.shape[-1]} words a block does not hold pages of head_dim={head_dim}, "
+        f"group_size={group_size}")
+    return P
+
+
+def _kv4(pool: Tensor, table: Tensor, head_dim: int, group_size: int) -> "_lib.KV4":
+    assert pool.is_cuda, "pool must be on a HIP device"
+    assert pool.dtype == torch.int32 and pool.dim() == 3 and pool.is_contiguous(), \
+        "pool must be contiguous int32 [pages, heads, words]"
+    assert table.dim() == 2, f"table must be [rows, max_pages], got {list(table.shape)}"
+    _int32(table, "table", tuple(table.shape), pool.device)
+    return _lib.KV4(pool.data_ptr(), table.data_ptr(), pool.shape[0], table.shape[0],
+                    table.shape[1], pool.shape[1], head_dim, group_size,
+                    _page_size(pool, head_dim, group_size))
+
+
+def _rope(q: Tensor, k: Tensor, v: Tensor | None, cos: Tensor, sin: Tensor, positions: Tensor,
+          q_weight: Tensor | None, k_weight: Tensor | None, eps: float,
+          interleaved: bool) -> "_lib.Rope":
+    _heads3(q, "q")
+    _heads3(k, "k", q)
+    T, Hq, D = q.shape
+    assert D in (64, 128, 256), f"head_dim must be 64, 128 or 256, got {D}"
+    dev = q.device
+    assert cos.dtype == torch.float32 and sin.dtype == torch.float32, "cos and sin must be fp32"
+    assert cos.dim() == 2 and cos.shape == sin.shape and cos.is_contiguous() and \
+        sin.is_contiguous(), "cos and sin must be contiguous [positions, rot_dim / 2]"
+    assert cos.device == dev and sin.device == dev, f"cos and sin must be on {dev}"
+    rot = 2 * cos.shape[1]
+    assert rot <= D and rot % 16 == 0, (
+        f"rot_dim={rot} (twice the tables' width) must be a multiple of 16 within head_dim={D}")
+    _int32(positions, "positions", (T,), dev)
+    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if w is not None:
+            assert w.shape == (D,) and w.dtype == q.dtype and w.is_contiguous() and \
+                w.device == dev, f"{name} must be contiguous [{D}] of the queries' type and device"
+    if v is not None:
+        _heads3(v, "v", q)
+        assert v.shape == k.shape, f"v must have the keys' shape {list(k.shape)}"
+    r = _lib.Rope()
+    r.q, r.q_token, r.q_head = q.data_ptr(), q.stride(0), q.stride(1)
+    r.k, r.k_token, r.k_head = k.data_ptr(), k.stride(0), k.stride(1)
+    if v is not None:
+        r.v, r.v_token, r.v_head = v.data_ptr(), v.stride(0), v.stride(1)
+    r.cos, r.sin, r.token_position = cos.data_ptr(), sin.data_ptr(), positions.data_ptr()
+    r.q_weight, r.k_weight = rt.ptr(q_weight), rt.ptr(k_weight)
+    r.tokens, r.positions = T, cos.shape[0]
+    r.q_heads, r.kv_heads, r.head_dim, r.rot_dim = Hq, k.shape[1], D, rot
+    r.eps = eps
+    r.flags = ((_lib.KV4_BF16 if q.dtype == torch.bfloat16 else 0)
+               | (_lib.KV4_INTERLEAVED if interleaved else 0))
+    return r
+
+
+def _dense(like: Tensor, heads: int, out: Tensor | None, name: str) -> Tensor:
+    shape = (like.shape[0], heads, like.shape[2])
+    if out is None:
+        return torch.empty(shape, dtype=like.dtype, device=like.device)
+    assert tuple(out.shape) == shape and out.dtype == like.dtype and out.is_contiguous() and \
+        out.device == like.device, f"{name} must be contiguous {list(shape)} of the queries' type"
+    return out
+
+
+def qk_norm_rope(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, positions: Tensor, *,
+                 q_weight: Tensor | None = None, k_weight: Tensor | None = None,
+                 eps: float = 1e-6, interleaved: bool = False,
+                 out: tuple[Tensor, Tensor] | None = None) -> tuple[Tensor, Tensor]:
+    """RMS norm of every query and key head, then the rotation of its first values.
+
+    Args:
+        q, k: [tokens, heads, head_dim], fp16 or bf16.
+        cos, sin: fp32 [positions, rot_dim / 2]; rot_dim a multiple of 16.
+        positions: int32 [tokens].  A position outside the tables gives NaN.
+        q_weight, k_weight: [head_dim]; ``None``: that side is not normed.
+        interleaved: values 2i, 2i + 1 rotate together, else i, i + rot_dim / 2.
+        out: optional (queries, keys) to write, contiguous.
+    Returns:
+        (queries, keys), computed in fp32 and rounded once.
+    """
+    r = _rope(q, k, None, cos, sin, positions, q_weight, k_weight, eps, interleaved)
+    qo = _dense(q, q.shape[1], out and out[0], "out[0]")
+    ko = _dense(q, k.shape[1], out and out[1], "out[1]")
+    r.q_out, r.k_out = qo.data_ptr(), ko.data_ptr()
+    with rt.on_device(q.device):
+        _lib.check(rt.lib().w4a16_qk_norm_rope(ctypes.byref(r), rt.stream_ptr(q.device)),
+                   "qk_norm_rope")
+    return qo, ko
+
+
+def kv4_append(q: Tensor, k: Tensor, v: Tensor, cos: Tensor, sin: Tensor, positions: Tensor,
+               pool: Tensor, table: Tensor, *, rows: Tensor | None = None, group_size: int = 64,
+               q_weight: Tensor | None = None, k_weight: Tensor | None = None, eps: float = 1e-6,
+               interleaved: bool = False, out: Tensor | None = None) -> Tensor:
+    """``qk_norm_rope`` with the keys and values stored in the cache instead.
+
+    Token i goes to position ``positions[i]`` of table row ``rows[i]`` (row i where
+    ``rows`` is None); one with a negative position, or one that the table has no
+    page for, is not stored.  No two tokens of a call may have the same place.
+    Returns the queries.
+    """
+    r = _rope(q, k, v, cos, sin, positions, q_weight, k_weight, eps, interleaved)
+    kv = _kv4(pool, table, q.shape[2], group_size)
+    assert pool.device == q.device, f"pool must be on {q.device}"
+    assert pool.shape[1] == k.shape[1], \
+        f"the pool has {pool.shape[1]} heads, the keys {k.shape[1]}"
+    if rows is not None:
+        _int32(rows, "rows", (q.shape[0],), q.device)
+    qo = _dense(q, q.shape[1], out, "out")
+    r.q_out = qo.data_ptr()
+    with rt.on_device(q.device):
+        _lib.check(rt.lib().w4a16_kv4_append(ctypes.byref(r), ctypes.byref(kv), rt.ptr(rows),
+                                             rt.stream_ptr(q.device)), "kv4_append")
+    return qo
+
+
+def kv4_read(pool: Tensor, table: Tensor, positions: Tensor, *, head_dim: int,
+             rows: Tensor | None = None, group_size: int = 64,
+             dtype: torch.dtype = torch.float16) -> tuple[Tensor, Tensor]:
+    """Stored tokens, (keys, values) [tokens, heads, head_dim]: the inverse of the
+    storing in ``kv4_append``.  Zeros for a place that the table does not hold."""
+    kv = _kv4(pool, table, head_dim, group_size)
+    assert dtype in _TYPES, f"dtype must be fp16 or bf16, got {dtype}"
+    assert positions.dim() == 1, f"positions must be [tokens], got {list(positions.shape)}"
+    T, dev = positions.shape[0], pool.device
+    _int32(positions, "positions", (T,), dev)
+    if rows is not None:
+        _int32(rows, "rows", (T,), dev)
+    k = torch.empty((T, pool.shape[1], head_dim), dtype=dtype, device=dev)
+    v = torch.empty_like(k)
+    with rt.on_device(dev):
+        _lib.check(rt.lib().w4a16_kv4_read(
+            ctypes.byref(kv), positions.data_ptr(), rt.ptr(rows), T, k.data_ptr(), v.data_ptr(),
+            _lib.KV4_BF16 if dtype == torch.bfloat16 else 0, rt.stream_ptr(dev)), "kv4_read")
+    return k, v
+
+
+def kv4_attention(q: Tensor, pool: Tensor, table: Tensor, lens: Tensor, *,
+                  q_starts: Tensor | None = None, seqs: Tensor | None = None,
+                  max_q: int | None = None, max_context: int | None = None,
+                  group_size: int = 64, scale: float | None = None, causal: bool = True,
+                  window: int = 0, return_lse: bool = False,
+                  out: Tensor | None = None) -> Tensor | tuple[Tensor, Tensor]:
+    """Attention of new tokens over the stored ones, the new ones among them.
+
+    Args:
+        q: [tokens, q_heads, head_dim]; q_heads a multiple of the pool's heads
+           (query head j uses head ``j // (q_heads // heads)``).
+        lens: int32 [rows of the table], tokens stored.
+        q_starts: int32 [batch + 1]: sequence b has tokens q_starts[b] ..
+           q_starts[b + 1] - 1 of q, the last ones of its ``lens``.  None: one
+           token a sequence.  Tokens of q that no sequence has are not computed.
+        seqs: int32 [batch], the table row of each sequence (None: row b).
+        max_q: the most tokens a sequence has in q (default: all of q's).  Tokens
+           beyond it are not computed.
+        max_context: the longest of the sequences, to size the launch by (default:
+           what a table row can hold).  Any value gives right results.
+        scale: of the scores, default 1 / sqrt(head_dim).
+        causal: a token at position p sees no later one; window > 0: only the last
+           ``window`` positions up to p.
+        return_lse: also the natural logarithm of the denominators, fp32 [tokens,
+           q_heads].
+        out: optional output, contiguous, of q's shape and type.
+    Returns:
+        [tokens, q_heads, head_dim]; zeros (lse -inf) for a token that sees nothing.
+    """
+    _heads3(q, "q")
+    T, Hq, D = q.shape
+    dev = q.device
+    kv = _kv4(pool, table, D, group_size)
+    assert pool.device == dev, f"pool must be on {dev}"
+    H = pool.shape[1]
+    assert H > 0 and Hq > 0 and Hq % H == 0, \
+        f"{Hq} query heads are not a multiple of the pool's {H}"
+    _int32(lens, "lens", (table.shape[0],), dev)
+    if q_starts is None:
+        batch = T
+        assert seqs is not None or T <= table.shape[0], \
+            f"{T} sequences, but the table has {table.shape[0]} rows"
+    else:
+        assert q_starts.dim() == 1 and q_starts.shape[0] > 0, "q_starts must be [batch + 1]"
+        batch = q_starts.shape[0] - 1
+        _int32(q_starts, "q_starts", (batch + 1,), dev)
+        assert seqs is not None or batch <= table.shape[0], \
+            f"{batch} sequences, but the table has {table.shape[0]} rows"
+    if seqs is not None:
+        _int32(seqs, "seqs", (batch,), dev)
+    assert window >= 0, f"window must not be negative, got {window}"
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    assert 0.0 < scale < 3e38, f"scale must be positive and finite, got {scale}"
+    most = table.shape[1] * kv.page_size
+    a = _lib.KV4Query()
+    a.q, a.q_token, a.q_head = q.data_ptr(), q.stride(0), q.stride(1)
+    a.lens, a.q_starts, a.seqs = lens.data_ptr(), rt.ptr(q_starts), rt.ptr(seqs)
+    a.tokens, a.batch = T, batch
+    a.max_q = T if max_q is None else max(0, int(max_q))
+    a.max_context = min(most if max_context is None else max(0, int(max_context)), 2**31 - 1)
+    a.q_heads, a.window, a.scale = Hq, min(int(window), 2**31 - 1), scale
+    a.flags = ((_lib.KV4_BF16 if q.dtype == torch.bfloat16 else 0)
+               | (_lib.KV4_CAUSAL if causal else 0))
+    y = _dense(q, Hq, out, "out")
+    a.out = y.data_ptr()
+    lse = torch.empty((T, Hq), dtype=torch.float32, device=dev) if return_lse else None
+    a.lse = rt.ptr(lse)
+    with rt.on_device(dev):
+        need = rt.lib().w4a16_kv4_attention_workspace_bytes(ctypes.byref(kv), ctypes.byref(a))
+        ws = rt.workspace(dev, need)
+        _lib.check(rt.lib().w4a16_kv4_attention(
+            ctypes.byref(kv), ctypes.byref(a), rt.ptr(ws), 0 if ws is None else ws.numel(),
+            rt.stream_ptr(dev)), "kv4_attention")
+    return (y, lse) if return_lse else y
+
+
+# ---- pages ---------------------------------------------------------------------
+
+def _pool4(pool: Tensor) -> tuple[int, int, int]:
+    """(layers, pages, words of a page) of a pool, one layer or all."""
+    assert pool.is_cuda, "pool must be on a HIP device"
+    assert pool.dtype == torch.int32 and pool.dim() in (3, 4) and pool.is_contiguous(), \
+        "pool must be contiguous int32 [pages, heads, words] or [layers, pages, heads, words]"
+    layers = pool.shape[0] if pool.dim() == 4 else 1
+    return layers, pool.shape[-3], pool.shape[-2] * pool.shape[-1]
+
+
+def _book(table: Tensor, lens: Tensor, refs: Tensor, page_size: int) -> "_lib.KV4Book":
+    assert table.is_cuda, "table must be on a HIP device"
+    assert table.dim() == 2, f"table must be [rows, max_pages], got {list(table.shape)}"
+    dev = table.device
+    _int32(table, "table", tuple(table.shape), dev)
+    _int32(lens, "lens", (table.shape[0],), dev)
+    assert refs.dim() == 1, f"refs must be [pages], got {list(refs.shape)}"
+    _int32(refs, "refs", tuple(refs.shape), dev)
+    assert page_size in (32, 64, 128, 256), \
+        f"page_size must be 32, 64, 128 or 256, got {page_size}"
+    return _lib.KV4Book(table.data_ptr(), lens.data_ptr(), refs.data_ptr(), table.shape[0],
+                        table.shape[1], refs.shape[0], page_size)
+
+
+def _list(t: Tensor, name: str, dev: torch.device, n: int | None = None) -> int:
+    assert t.dim() == 1, f"{name} must be a list [n], got {list(t.shape)}"
+    _int32(t, name, (t.shape[0] if n is None else n,), dev)
+    assert t.shape[0] <= 1 << 20, f"{name} has {t.shape[0]} entries, at most {1 << 20}"
+    return t.shape[0]
+
+
+def _status(status: Tensor | None, dev: torch.device) -> Tensor:
+    if status is None:
+        return torch.zeros(1, dtype=torch.int32, device=dev)
+    return _int32(status, "status", (1,), dev)
+
+
+def kv4_copy_pages(pool: Tensor, src: Tensor, dst: Tensor) -> None:
+    """Page ``src[i]`` to page ``dst[i]`` in every layer of ``pool``; no page of
+    ``dst`` is named twice or is in ``src``.  Pairs outside the pool are skipped."""
+    layers, pages, words = _pool4(pool)
+    dev = pool.device
+    n = _list(src, "src", dev)
+    _list(dst, "dst", dev, n)
+    with rt.on_device(dev):
+        _lib.check(rt.lib().w4a16_kv4_copy_pages(pool.data_ptr(), layers, pages, words,
+                                                 src.data_ptr(), dst.data_ptr(), n,
+                                                 rt.stream_ptr(dev)), "kv4_copy_pages")
+
+
+def kv4_extend(table: Tensor, lens: Tensor, refs: Tensor, seqs: Tensor, counts: Tensor, *,
+               page_size: int, status: Tensor | None = None) -> Tensor:
+    """Room for ``counts[i]`` more tokens in row ``seqs[i]`` (each row named once):
+    the lowest free pages in the list's order, ``lens`` grown by the counts.
+
+    ``status`` (int32 [1], kept by the caller; a new one otherwise) gathers
+    ``KV4Cache.NO_PAGES``, ``ROW_FULL`` and ``BAD_ROW``; such a row is unchanged.
+    Returned, so that a caller may look when it next waits for the device.
+    """
+    book = _book(table, lens, refs, page_size)
+    dev = table.device
+    n = _list(seqs, "seqs", dev)
+    _list(counts, "counts", dev, n)
+    with rt.on_device(dev):
+        status = _status(status, dev)
+        _lib.check(rt.lib().w4a16_kv4_extend(ctypes.byref(book), seqs.data_ptr(),
+                                             counts.data_ptr(), n, status.data_ptr(),
+                                             rt.stream_ptr(dev)), "kv4_extend")
+    return status
+
+
+def kv4_fork(pool: Tensor, table: Tensor, lens: Tensor, refs: Tensor, parents: Tensor,
+             children: Tensor, *, page_size: int, status: Tensor | None = None) -> Tensor:
+    """Row ``children[i]`` (empty, named once) becomes a copy of row ``parents[i]``:
+    whole pages are shared, a partly filled last page is copied, in every layer, to
+    the lowest free one.  Returns the status (see ``kv4_extend``)."""
+    layers, pages, words = _pool4(pool)
+    book = _book(table, lens, refs, page_size)
+    dev = pool.device
+    assert table.device == dev, f"table must be on {dev}"
+    assert refs.shape[0] == pages, f"refs has {refs.shape[0]} pages, the pool {pages}"
+    n = _list(parents, "parents", dev)
+    _list(children, "children", dev, n)
+    with rt.on_device(dev):
+        status = _status(status, dev)
+        ws = rt.workspace(dev, rt.lib().w4a16_kv4_fork_workspace_bytes(n))
+        _lib.check(rt.lib().w4a16_kv4_fork(
+            pool.data_ptr(), layers, words, ctypes.byref(book), parents.data_ptr(),
+            children.data_ptr(), n, status.data_ptr(), rt.ptr(ws),
+            0 if ws is None else ws.numel(), rt.stream_ptr(dev)), "kv4_fork")
+    return status
+
+
+def kv4_free(table: Tensor, lens: Tensor, refs: Tensor, seqs: Tensor) -> None:
+    """Empty rows ``seqs``; a page that no other row holds is free afterwards."""
+    book = _book(table, lens, refs, 32)   # (whatever a page holds)
+    dev = table.device
+    n = _list(seqs, "seqs", dev)
+    with rt.on_device(dev):
+        _lib.check(rt.lib().w4a16_kv4_free(ctypes.byref(book), seqs.data_ptr(), n,
+                                           rt.stream_ptr(dev)), "kv4_free")
+
+
+def kv4_compact(pool: Tensor, table: Tensor, refs: Tensor) -> tuple[Tensor, Tensor, Tensor]:
+    """Move the pages in use to the front of ``pool``, in place and in every layer:
+    with ``live`` pages in use, the k-th that lies at or beyond ``live`` goes to the
+    k-th free one below.  Returns (table, refs, live): the new table and use counts
+    (new tensors) and int32 [1]."""
+    layers, pages, words = _pool4(pool)
+    dev = pool.device
+    assert table.dim() == 2, f"table must be [rows, max_pages], got {list(table.shape)}"
+    _int32(table, "table", tuple(table.shape), dev)
+    _int32(refs, "refs", (pages,), dev)
+    assert pages > 0, "the pool has no pages"
+    with rt.on_device(dev):
+        new_table, new_refs = torch.empty_like(table), torch.empty_like(refs)
+        live = torch.empty(1, dtype=torch.int32, device=dev)
+        # (rows' lengths do not change: any array stands for them)
+        book = _lib.KV4Book(table.data_ptr(), refs.data_ptr(), refs.data_ptr(), table.shape[0],
+                            table.shape[1], pages, 32)
+        ws = rt.workspace(dev, rt.lib().w4a16_kv4_compact_workspace_bytes(pages))
+        _lib.check(rt.lib().w4a16_kv4_compact(
+            pool.data_ptr(), layers, words, ctypes.byref(book), new_table.data_ptr(),
+            new_refs.data_ptr(), live.data_ptr(), rt.ptr(ws), 0 if ws is None else ws.numel(),
+            rt.stream_ptr(dev)), "kv4_compact")
+    return new_table, new_refs, live

@@ -58,7 +58,7 @@ Kv4Plan kv4_attention_plan(const w4a16_kv4& kv, const w4a16_kv4_query& q) {
   const int per_kv = q.q_heads / kv.heads;
   const int64_t rows = q.max_q * per_kv;
   p.rows_form = rows > 32;
-  p.cols = rows > 16 ? 2 : 1;
+  p.cols = rows > 16 && kv.head_dim < 256 ? 2 : 1;
   const int64_t tile_rows = p.rows_form ? 64 * p.cols : 16 * p.cols;
   p.tiles = (int)((rows + tile_rows - 1) / tile_rows);
   int64_t span = q.max_context;
@@ -113,7 +113,8 @@ hipError_t launch_kv4_attention(const Kv4Attn& c, hipStream_t st) {
   a.bf16 = (q.flags & W4A16_KV4_BF16) != 0;
   a.vec = (reinterpret_cast<uintptr_t>(q.q) & 15) == 0 && (q.q_token | q.q_head) % 8 == 0;
   const int D = kv.head_dim, NG = D / kv.group_size;
-  const hipError_t e = c.rows_form   ? launch_attention_rows(a, D, NG, st)
+  const hipError_t e = c.rows_form && D == 256 ? launch_attention_rows256(a, NG, st)
+                       : c.rows_form ? launch_attention_rows(a, D, NG, st)
                        : c.cols == 2 ? launch_attention_tokens2(a, D, NG, st)
                                      : launch_attention_tokens1(a, D, NG, st);
   if (e != hipSuccess || c.splits == 1) return e;

@@ -83,6 +83,10 @@ __device__ __forceinline__ AttnSpan attn_span(const AttnArgs& a, int b, int r0, 
   return s;
 }
 
+typedef __attribute__((address_space(3))) uint32_t lds_dword;
+typedef __attribute__((address_space(1))) uint32_t glb_dword;
+typedef __attribute__((address_space(4))) int32_t const_dword;   // read by scalar loads
+
 // Combining two halves / four rows of a wave: every lane gets op over the lanes
 // that share its l % 16.
 template <class F>
@@ -121,46 +125,90 @@ __device__ __forceinline__ f16x8 value_halves(uint32_t w, const MagicRegs& mg) {
 __device__ __forceinline__ float lo_f32(uint32_t w) { return (float)as_h((uint16_t)w); }
 __device__ __forceinline__ float hi_f32(uint32_t w) { return (float)as_h((uint16_t)(w >> 16)); }
 
-// One lane's words of 32 tokens: keys and values, with the group words of the
-// eight tokens that its scores belong to.
+// 32 tokens of a page as they lie in LDS, brought there by LDS-direct loads of 16
+// bytes a lane (codes) and 4 (group words).  Each lane fetches the codes that it
+// will unpack itself, so its reads are free of bank conflicts; a group word is read
+// by the sixteen lanes of its tokens at once.
 template <int D, int NG>
-struct KvBlock {
-  uint32_t k[2][D / 32], v[D / 16], kg[NG][8], vg[NG][8];
-};
+struct Stage {
+  static constexpr int kCodeLoads = D / 64;               // of 1 KB, keys and values each
+  static constexpr int kLoads = 2 * kCodeLoads + NG;
+  static constexpr int kGroups = 512 * kCodeLoads;        // first group word
+  static constexpr int kWords = kGroups + 64 * NG;
 
-template <int N>
-__device__ __forceinline__ void load_words(uint32_t* dst, const uint32_t* p) {
-  if constexpr (N == 2) {
-    const u32x2 v = *reinterpret_cast<const u32x2*>(p);
-    dst[0] = v.x;
-    dst[1] = v.y;
-  } else {
+  // Word offsets of a lane's first key load, value load and group load in a block.
+  int key, value, group;
+  __device__ __forceinline__ Stage(int P, int lane) {
+    const int c = lane & 15, g = lane >> 4;
+    if constexpr (D == 64) {
+      const int j = lane >> 5, cc = (lane & 31) >> 1;     // both tiles in one load
+      key = (8 * (cc >> 2) + 4 * j + (cc & 3)) * (D / 8) + 4 * (lane & 1);
+    } else {
+      key = (8 * (c >> 2) + (c & 3)) * (D / 8) + g * (D / 32);
+    }
+    value = P * (D / 8 + NG) + g * D + 4 * c;
+    group = lane < 32 ? P * (D / 8) + lane : P * (D / 4 + NG) + lane - 32;
+  }
+  // Load q of kLoads of the 32 tokens from t0 on of block `blk`.
+  __device__ __forceinline__ void load(int q, const uint32_t* blk, int P, int t0,
+                                       uint32_t* lds) const {
+    const uint32_t* from;
+    if (q < kCodeLoads) {
+      const int j = D == 256 ? q >> 1 : q, half = D == 256 ? q & 1 : 0;
+      from = blk + t0 * (D / 8) + key + j * (D / 2) + 4 * half;
+    } else if (q < 2 * kCodeLoads) {
+      from = blk + t0 * (D / 8) + value + 64 * (q - kCodeLoads);
+    } else {
+      from = blk + t0 + group + (q - 2 * kCodeLoads) * P;
+    }
+    lds_dword* to = (lds_dword*)(lds + (q < 2 * kCodeLoads ? 256 * q
+                                                           : kGroups + 64 * (q - 2 * kCodeLoads)));
+    if (q < 2 * kCodeLoads)
+      __builtin_amdgcn_global_load_lds((const glb_dword*)from, to, 16, 0, 0);
+    else
+      __builtin_amdgcn_global_load_lds((const glb_dword*)from, to, 4, 0, 0);
+  }
+
+  // What a lane reads back: the words of key tile j, four value words, the eight
+  // group words of its tokens.
+  static __device__ __forceinline__ void keys(const uint32_t* lds, int j, int lane,
+                                              uint32_t w[D / 32]) {
+    if constexpr (D == 64) {
+      const u32x2 v = *reinterpret_cast<const u32x2*>(
+          lds + 128 * j + 8 * (lane & 15) + 2 * (lane >> 4));
+      w[0] = v.x;
+      w[1] = v.y;
+    } else {
 #pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      const u32x4 v = *reinterpret_cast<const u32x4*>(p + i);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) dst[i + j] = v[j];
+      for (int h = 0; h < D / 128; ++h) read4(lds + 256 * (j * (D / 128) + h) + 4 * lane, w + 4 * h);
     }
   }
-}
+  static __device__ __forceinline__ void values(const uint32_t* lds, int h, int lane,
+                                                uint32_t w[4]) {
+    read4(lds + 256 * (kCodeLoads + h) + 4 * lane, w);
+  }
+  static __device__ __forceinline__ void key_groups(const uint32_t* lds, int n, int lane,
+                                                    uint32_t w[8]) {
+    read4(lds + kGroups + 64 * n + 8 * (lane >> 4), w);
+    read4(lds + kGroups + 64 * n + 8 * (lane >> 4) + 4, w + 4);
+  }
+  static __device__ __forceinline__ void value_groups(const uint32_t* lds, int n, int lane,
+                                                      uint32_t w[8]) {
+    read4(lds + kGroups + 64 * n + 32 + 8 * (lane >> 4), w);
+    read4(lds + kGroups + 64 * n + 36 + 8 * (lane >> 4), w + 4);
+  }
+  static __device__ __forceinline__ void read4(const uint32_t* p, uint32_t w[4]) {
+    const u32x4 v = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = v[i];
+  }
+};
 
-template <int D, int NG>
-__device__ __forceinline__ void load_block(KvBlock<D, NG>& x, const uint32_t* blk, int P, int t0,
-                                           int lane) {
-  const int c = lane & 15, g = lane >> 4;
-  const uint32_t* codes = blk + t0 * (D / 8);
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-    load_words<D / 32>(x.k[j], codes + (8 * (c >> 2) + 4 * j + (c & 3)) * (D / 8) + g * (D / 32));
-#pragma unroll
-  for (int n = 0; n < NG; ++n)
-    load_words<8>(x.kg[n], blk + P * (D / 8) + n * P + t0 + 8 * g);
-#pragma unroll
-  for (int h = 0; h < D / 64; ++h)
-    load_words<4>(x.v + 4 * h, codes + P * (D / 8 + NG) + g * D + 64 * h + 4 * c);
-#pragma unroll
-  for (int n = 0; n < NG; ++n)
-    load_words<8>(x.vg[n], blk + P * (D / 4 + NG) + n * P + t0 + 8 * g);
+// Waits until at most N of the wave's loads are under way.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(N >= 0 && N <= 63, "s_waitcnt's counter");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
 template <int D, int NG, int C>
@@ -199,17 +247,24 @@ struct AttnWave {
     see_lo[c] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
     const uint16_t* src = a.q + (int64_t)(s.q0 + (there ? i : 0)) * a.q_token +
                           (int64_t)(h * a.per_kv + (there ? hh : 0)) * a.q_head;
-    float x[kSteps][8], most = 0.0f;
+    u32x4 x[kSteps];
+    float most = 0.0f;
+    auto value = [&](int k, int j) {
+      const uint16_t u = (uint16_t)(x[k][j / 2] >> (16 * (j & 1)));
+      return a.bf16 ? to_f32<true>(u) : to_f32<false>(u);
+    };
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
-      const u32x4 w = there ? load8(src + 32 * k + 8 * g, a.vec) : u32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint16_t u = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
-        x[k][j] = a.bf16 ? to_f32<true>(u) : to_f32<false>(u);
-        most = fmaxf(most, fabsf(x[k][j]));
-      }
+      x[k] = u32x4{0, 0, 0, 0};
+      if (there) x[k] = load8(src + 32 * k + 8 * g, a.vec);
     }
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(value(k, j)));
+    // (converted anew below: half the registers)
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) asm volatile("" : "+v"(x[k]));
     most = max_rows(most);
     // 2^e brings the largest value into [2^14, 2^15)
     int e = 0;
@@ -220,7 +275,7 @@ struct AttnWave {
     for (int k = 0; k < kSteps; ++k)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float y = ldexpf(x[k][j], e);
+        const float y = ldexpf(value(k, j), e);
         Q[c][k / (kSteps / NG)] += y;
         q[c][k][j] = (f16)(j & 2 ? y * 0.0625f : y);
       }
@@ -229,14 +284,18 @@ struct AttnWave {
     fac[c] = ldexpf(a.scale_log2, 24 - e);
   }
 
-  // 32 tokens from t on.  kMask: some of them are hidden from some row, or lie at
-  // or beyond n.
-  template <bool kMask>
-  __device__ __forceinline__ void step(const KvBlock<D, NG>& x, int t, int lane) {
+  // 32 tokens from t on.  `mask`: some of them are hidden from some row.
+  __device__ __forceinline__ void step(const uint32_t* lds, int t, int lane, bool mask) {
+    typedef Stage<D, NG> S;
     const int g = lane >> 4, mine = t + 8 * g;
     float sc[C][8];
+    uint32_t kg[NG][8], vg[NG][8];
+#pragma unroll
+    for (int n = 0; n < NG; ++n) S::key_groups(lds, n, lane, kg[n]);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
+      uint32_t kw[kSteps];
+      S::keys(lds, j, lane, kw);
       f32x4 s[C][NG];
 #pragma unroll
       for (int c = 0; c < C; ++c)
@@ -247,7 +306,7 @@ struct AttnWave {
         }
 #pragma unroll
       for (int k = 0; k < kSteps; ++k) {
-        const f16x8 w = code_halves(x.k[j][k]);
+        const f16x8 w = code_halves(kw[k]);
 #pragma unroll
         for (int c = 0; c < C; ++c)
           s[c][k / (kSteps / NG)] =
@@ -260,14 +319,27 @@ struct AttnWave {
           float v = 0.0f;
 #pragma unroll
           for (int n = 0; n < NG; ++n) {
-            const float u = hi_f32(x.kg[n][4 * j + r]) * Q[c][n];
-            v = fmaf(lo_f32(x.kg[n][4 * j + r]), s[c][n][r], n ? v + u : u);
-          }
-          if constexpr (kMask) {
-            const int tt = mine + 4 * j + r;
-            v = tt >= see_lo[c] && tt < see_hi[c] ? v : -__builtin_inff();
+            v = fmaf(hi_f32(kg[n][4 * j + r]), Q[c][n], v);
+            v = fmaf(lo_f32(kg[n][4 * j + r]), s[c][n][r], v);
           }
           sc[c][4 * j + r] = v;
+        }
+    }
+    auto hidden = [&](int c, int i) { return mine + i < see_lo[c] || mine + i >= see_hi[c]; };
+    if (mask) {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sc[c][i] = hidden(c, i) ? -__builtin_inff() : sc[c][i];
+    }
+#pragma unroll
+    for (int n = 0; n < NG; ++n) S::value_groups(lds, n, lane, vg[n]);
+    if (mask) {   // what no row sees may hold anything
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (mine + i < any_lo || mine + i >= any_hi) {
+#pragma unroll
+          for (int n = 0; n < NG; ++n) vg[n][i] = 0;
         }
     }
     float big = 0.0f, sv[NG][8];
@@ -276,11 +348,8 @@ struct AttnWave {
     for (int n = 0; n < NG; ++n)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        float s = fmaf(lo_f32(x.vg[n][i]), f, 0.0f);
-        // what no row sees may hold anything
-        if constexpr (kMask) s = mine + i >= any_lo && mine + i < any_hi ? s : 0.0f;
-        sv[n][i] = s;
-        big = fmaxf(big, s);
+        sv[n][i] = fmaf(lo_f32(vg[n][i]), f, 0.0f);
+        big = fmaxf(big, sv[n][i]);
       }
     float top[C];
     bool move = !(big <= 128.0f);
@@ -326,43 +395,56 @@ struct AttnWave {
       for (int i = 0; i < 8; ++i) {
         const float p = __builtin_amdgcn_exp2f(fmaf(sc[c][i], fac[c], -m[c]));
         l[c] += p;
-        const bool hidden = kMask && (mine + i < see_lo[c] || mine + i >= see_hi[c]);
-#pragma unroll
-        for (int n = 0; n < NG; ++n) {
-          const float z = p * sv[n][i];
-          w[c][n][i] = (f16)(hidden ? 0.0f : z);
-          const float u = fmaf(p, hi_f32(x.vg[n][i]), csum[c][n]);
-          csum[c][n] = hidden ? csum[c][n] : u;
-        }
+        sc[c][i] = p;
       }
-#pragma unroll
-    for (int i = 0; i < kTiles; ++i) {
-      const f16x8 v = value_halves(x.v[i], mg);
+    if (mask) {   // a token that one row sees may spoil only that one
 #pragma unroll
       for (int c = 0; c < C; ++c)
-        acc[c][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[c][i / (kTiles / NG)], acc[c][i],
-                                                           0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const bool gone = hidden(c, i);
+#pragma unroll
+          for (int n = 0; n < NG; ++n) {
+            w[c][n][i] = (f16)(gone ? 0.0f : sc[c][i] * sv[n][i]);
+            csum[c][n] = fmaf(sc[c][i], gone ? 0.0f : hi_f32(vg[n][i]), csum[c][n]);
+          }
+        }
+    } else {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int n = 0; n < NG; ++n) {
+            w[c][n][i] = (f16)(sc[c][i] * sv[n][i]);
+            csum[c][n] = fmaf(sc[c][i], hi_f32(vg[n][i]), csum[c][n]);
+          }
+    }
+#pragma unroll
+    for (int h = 0; h < D / 64; ++h) {
+      uint32_t vw[4];
+      S::values(lds, h, lane, vw);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f16x8 v = value_halves(vw[j], mg);
+        const int i = 4 * h + j;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+          acc[c][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[c][i / (kTiles / NG)], acc[c][i],
+                                                             0, 0, 0);
+      }
     }
   }
 
-  // Blocks first, first + stride, ... below end.  Every one of the wave's rows sees
-  // the tokens [all_lo, all_hi), none sees others than [any_lo, any_hi).
+  // Every one of the wave's rows sees the tokens [all_lo, all_hi), none sees others
+  // than [any_lo, any_hi).
   int all_lo, all_hi, any_lo, any_hi;
-  __device__ __forceinline__ void run(const AttnArgs& a, const AttnSpan& s, int h, int first,
-                                      int end, int stride, int lane) {
-    const int P = 1 << a.page_shift, words = P * (D / 4 + 2 * NG);
-    const int32_t* pages = a.table + (int64_t)s.row * a.max_pages;
-    for (int kb = first; kb < end; kb += stride) {
-      const int t = kb << 5;
-      const int page = __builtin_amdgcn_readfirstlane(pages[t >> a.page_shift]);
-      if ((uint32_t)page >= (uint32_t)a.pages) continue;   // a missing page: its tokens are hidden
-      KvBlock<D, NG> x;
-      load_block(x, a.pool + ((int64_t)page * a.heads + h) * words, P, t & (P - 1), lane);
-      if (t < all_lo || t + 32 > all_hi)
-        step<true>(x, t, lane);
-      else
-        step<false>(x, t, lane);
-    }
+
+  // Block kb, in LDS; `there`: its page exists.
+  __device__ __forceinline__ void block(const uint32_t* lds, int kb, bool there, int lane) {
+    const int t = kb << 5;
+    if (!there || t >= any_hi || t + 32 <= any_lo) return;
+    step(lds, t, lane, t < all_lo || t + 32 > all_hi);
   }
 
   // Sums over all the wave's tokens; then value d = 16 i + 4 (lane / 16) + j of the
@@ -405,13 +487,43 @@ __device__ __forceinline__ float lse_of(float m, float l) {
   return l > 0.0f || l != l ? (m + log2f(l)) * 0.6931471805599453f : -__builtin_inff();
 }
 
-// kRows false: the four waves share 16 * C rows and take blocks in turn; true: each
-// has 16 * C rows of its own.  Grid: kv head fastest (an XCD then keeps to few heads
-// and finds their codes in its L2), then split, sequence, and the row tiles from the
-// last, which sees the most tokens, to the first.
+// Pages of a row's blocks.
+struct PageOf {
+  const const_dword* row;
+  int shift, pages;
+  // (block kb's page; -1: missing)
+  __device__ __forceinline__ int operator()(int kb) const {
+    const int p = row[kb >> (shift - 5)];
+    return (uint32_t)p < (uint32_t)pages ? p : -1;
+  }
+};
+
+// Buffers of 32 tokens a wave (or, rows form, of 64 a workgroup) that are filled in
+// turn.  Three, so that two are on their way while one is worked on; two for heads
+// of 256, where three leave a CU one workgroup.
+template <int D>
+constexpr int kStages = D == 256 ? 2 : 3;
+
+// kRows false: the four waves share 16 * C rows and take blocks of 32 tokens in turn,
+// each through buffers of its own; true: each has 16 * C rows of its own, and all
+// go through the workgroup's blocks together, 64 tokens at a time.  Grid: kv head
+// fastest (an XCD then keeps to few heads and finds their codes in its L2), then
+// split, sequence, and the row tiles from the last, which sees the most tokens, to
+// the first.
+// Waves per SIMD that the registers allow without spilling.  Nothing may spill: the
+// loop's counted waits take every load for one of its own.
+template <int D, int NG, int C>
+constexpr int kWaves = C * (D + 32 * (NG - 1)) <= 320 ? 2 : 1;
+
 template <int D, int NG, int C, bool kRows>
-__global__ __launch_bounds__(kAttnThreads) void kv4_attention_kernel(const AttnArgs a) {
-  constexpr int kTiles = D / 16;
+__global__ __launch_bounds__(kAttnThreads, (kWaves<D, NG, C>)) void kv4_attention_kernel(const AttnArgs a) {
+  typedef Stage<D, NG> S;
+  constexpr int kTiles = D / 16, kS = kStages<D>;
+  constexpr int kRing = kRows ? kS * 2 * S::kWords : 4 * kS * S::kWords;
+  // the four waves' results (rows 4 floats apart beyond D: the four groups of lanes
+  // use different banks), then their maxima and denominators
+  constexpr int kSumRow = D + 4, kSum = kRows ? 0 : 4 * 16 * kSumRow + 4 * 16 * 2;
+  __shared__ __attribute__((aligned(16))) uint32_t lds[kRing > kSum ? kRing : kSum];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint32_t id = blockIdx.x;
   const int h = id % a.heads;
@@ -426,25 +538,101 @@ __global__ __launch_bounds__(kAttnThreads) void kv4_attention_kernel(const AttnA
   if (r0 >= R) return;
   if (a.splits > 1 && split >= s.active) return;
   const int w0 = kRows ? r0 + wave * 16 * C : r0;   // the wave's first row
-  if (kRows && w0 >= R) return;
 
   AttnWave<D, NG, C> w;
   w.start();
 #pragma unroll
   for (int c = 0; c < C; ++c) w.load_row(a, s, h, w0 + 16 * c + (lane & 15), c, lane);
+  // (rows past the last query see nothing, and need no mask to be ignored)
+  const int p0 = s.n - s.nq + w0 / a.per_kv;   // positions of the first and last query
+  const int p1 = s.n - s.nq + min((w0 + 16 * C - 1) / a.per_kv, s.nq - 1);
+  w.all_hi = a.causal ? min(max(p0 + 1, 0), s.n) : s.n;
+  w.any_hi = a.causal ? min(max(p1 + 1, 0), s.n) : s.n;
+  w.any_lo = a.window > 0 ? min(max(0, p0 - a.window + 1), w.any_hi) : 0;
+  w.all_lo = a.window > 0 ? max(0, p1 - a.window + 1) : 0;
+  if (w0 >= R) w.any_hi = 0;
   {
-    const int i0 = w0 / a.per_kv, i1 = min((w0 + 16 * C - 1) / a.per_kv, s.nq - 1);
-    // (rows past the last query see nothing, and need no mask to be ignored)
-    const int p0 = s.n - s.nq + i0, p1 = s.n - s.nq + i1;   // positions of first and last query
-    w.all_hi = a.causal ? min(max(p0 + 1, 0), s.n) : s.n;
-    w.any_hi = a.causal ? min(max(p1 + 1, 0), s.n) : s.n;
-    w.any_lo = a.window > 0 ? min(max(0, p0 - a.window + 1), w.any_hi) : 0;
-    w.all_lo = a.window > 0 ? max(0, p1 - a.window + 1) : 0;
-    // the split's blocks, as far as the wave's own rows see them
-    int first = s.first + split * a.chunk, end = (w.any_hi + 31) >> 5;
-    if (split + 1 < s.active) end = min(end, first + a.chunk);
-    if (kRows) first = max(first, w.any_lo >> 5);
-    w.run(a, s, h, kRows ? first : first + wave, end, kRows ? 1 : 4, lane);
+    // the split's blocks
+    const int first = s.first + split * a.chunk;
+    int end = (s.hi + 31) >> 5;
+    if (split + 1 < s.active) end = first + a.chunk;
+    if (a.pages == 0) end = first;
+    const int P = 1 << a.page_shift, words = P * (D / 4 + 2 * NG);
+    const PageOf page{(const const_dword*)(a.table + (int64_t)max(s.row, 0) * a.max_pages),
+                      a.page_shift, a.pages};
+    const S stage(P, lane);
+    auto block = [&](int pg, int kb) {   // (a missing page's loads go to page 0, unused)
+      return a.pool + ((int64_t)max(pg, 0) * a.heads + h) * words;
+    };
+    if constexpr (kRows) {
+      // wave w makes loads w, w + 4, ... of a pair of blocks; the last again where
+      // they do not come out even, so that all waves count the same
+      constexpr int kPair = 2 * S::kLoads, kMine = (kPair + 3) / 4;
+      uint32_t there = 0;   // two bits a buffer
+      auto fill = [&](int slot, int kb) {
+        const int k1 = min(kb + 1, end - 1);
+        const int pg0 = page(kb), pg1 = page(k1);
+        there = (there & ~(3u << (2 * slot))) |
+                ((pg0 >= 0 ? 1u : 0u) | (pg1 >= 0 && kb + 1 < end ? 2u : 0u)) << (2 * slot);
+        const uint32_t *b0 = block(pg0, kb), *b1 = block(pg1, k1);
+        uint32_t* to = lds + slot * 2 * S::kWords;
+#pragma unroll
+        for (int i = 0; i < kPair; ++i)
+          if (i % 4 == wave || (i == kPair - 1 && kPair % 4 && wave >= kPair % 4))
+            stage.load(i % S::kLoads, i < S::kLoads ? b0 : b1, P,
+                       ((i < S::kLoads ? kb : k1) << 5) & (P - 1),
+                       to + (i < S::kLoads ? 0 : S::kWords));
+      };
+#pragma unroll
+      for (int i = 0; i < kS - 1; ++i)
+        if (first + 2 * i < end) fill(i, first + 2 * i);
+      int slot = 0;
+      for (int kb = first; kb < end; kb += 2) {
+        // this pair is there, by every wave's loads, and the last one read by all
+        if (kS == 3 && kb + 2 < end)
+          wait_loads<kMine>();
+        else
+          wait_loads<0>();
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        const int last = slot == 0 ? kS - 1 : slot - 1;
+        if (kb + 2 * (kS - 1) < end) fill(last, kb + 2 * (kS - 1));
+        const uint32_t* x = lds + slot * 2 * S::kWords;
+        w.block(x, kb, there >> (2 * slot) & 1, lane);
+        w.block(x + S::kWords, kb + 1, there >> (2 * slot) & 2, lane);
+        slot = slot + 1 == kS ? 0 : slot + 1;
+      }
+    } else {
+      uint32_t* mine = lds + wave * kS * S::kWords;
+      uint32_t there = 0;
+      auto fill = [&](int slot, int kb) {
+        const int pg = page(kb);
+        there = (there & ~(1u << slot)) | (pg >= 0 ? 1u : 0u) << slot;
+        const uint32_t* from = block(pg, kb);
+#pragma unroll
+        for (int i = 0; i < S::kLoads; ++i)
+          stage.load(i, from, P, (kb << 5) & (P - 1), mine + slot * S::kWords);
+      };
+#pragma unroll
+      for (int i = 0; i < kS - 1; ++i)
+        if (first + wave + 4 * i < end) fill(i, first + wave + 4 * i);
+      int slot = 0;
+      for (int kb = first + wave; kb < end; kb += 4) {
+        const int last = slot == 0 ? kS - 1 : slot - 1;
+        const int ahead = kb + 4 * (kS - 1);
+        if (ahead < end) {
+          // (what was read of this buffer has been used: its last values fed products)
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          fill(last, ahead);
+          wait_loads<(kS - 1) * S::kLoads>();
+        } else if (kS == 3 && kb + 4 < end) {
+          wait_loads<S::kLoads>();
+        } else {
+          wait_loads<0>();
+        }
+        w.block(mine + slot * S::kWords, kb, there >> slot & 1, lane);
+        slot = slot + 1 == kS ? 0 : slot + 1;
+      }
+    }
   }
   w.finish();
 
@@ -479,9 +667,9 @@ __global__ __launch_bounds__(kAttnThreads) void kv4_attention_kernel(const AttnA
       }
     }
   } else {
-    // (rows 4 floats apart beyond D: the four groups of lanes use different banks)
-    __shared__ float sum[4][16][D + 4];
-    __shared__ float ml[4][16][2];
+    float (*sum)[16][kSumRow] = reinterpret_cast<float(*)[16][kSumRow]>(lds);
+    float (*ml)[16][2] = reinterpret_cast<float(*)[16][2]>(lds + 4 * 16 * kSumRow);
+    __syncthreads();   // the buffers have been read
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       if (c) __syncthreads();
@@ -538,20 +726,28 @@ __global__ __launch_bounds__(kAttnThreads) void kv4_attention_kernel(const AttnA
 template <int C, bool kRows>
 hipError_t launch_attention_form(const AttnArgs& a, int D, int NG, hipStream_t st) {
   const dim3 grid((unsigned)a.heads * a.splits * a.batch * a.tiles), block(kAttnThreads);
-  switch (D * 8 + NG) {
+  switch (D == 256 ? 0 : D * 8 + NG) {
     case 64 * 8 + 1: kv4_attention_kernel<64, 1, C, kRows><<<grid, block, 0, st>>>(a); break;
     case 64 * 8 + 2: kv4_attention_kernel<64, 2, C, kRows><<<grid, block, 0, st>>>(a); break;
     case 128 * 8 + 1: kv4_attention_kernel<128, 1, C, kRows><<<grid, block, 0, st>>>(a); break;
     case 128 * 8 + 2: kv4_attention_kernel<128, 2, C, kRows><<<grid, block, 0, st>>>(a); break;
     case 128 * 8 + 4: kv4_attention_kernel<128, 4, C, kRows><<<grid, block, 0, st>>>(a); break;
-    case 256 * 8 + 1: kv4_attention_kernel<256, 1, C, kRows><<<grid, block, 0, st>>>(a); break;
-    case 256 * 8 + 2: kv4_attention_kernel<256, 2, C, kRows><<<grid, block, 0, st>>>(a); break;
-    default: kv4_attention_kernel<256, 4, C, kRows><<<grid, block, 0, st>>>(a); break;
+    default:
+      if constexpr (C == 1) {   // (two columns of heads of 256 do not fit the registers)
+        switch (NG) {
+          case 1: kv4_attention_kernel<256, 1, 1, kRows><<<grid, block, 0, st>>>(a); break;
+          case 2: kv4_attention_kernel<256, 2, 1, kRows><<<grid, block, 0, st>>>(a); break;
+          default: kv4_attention_kernel<256, 4, 1, kRows><<<grid, block, 0, st>>>(a); break;
+        }
+        break;
+      }
+      return hipErrorInvalidValue;
   }
   return hipGetLastError();
 }
 hipError_t launch_attention_tokens1(const AttnArgs& a, int D, int NG, hipStream_t st);
 hipError_t launch_attention_tokens2(const AttnArgs& a, int D, int NG, hipStream_t st);
 hipError_t launch_attention_rows(const AttnArgs& a, int D, int NG, hipStream_t st);
+hipError_t launch_attention_rows256(const AttnArgs& a, int NG, hipStream_t st);
 
 }  // namespace w4a16

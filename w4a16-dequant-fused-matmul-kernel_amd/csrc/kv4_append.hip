@@ -45,7 +45,7 @@ struct RopeArgs {
   int group_lanes, NG;                              // lanes of D / 8 that share a group
   int chunk, value_blocks, qk_blocks;
   float eps;
-  bool interleaved, vec, store;
+  bool interleaved, store;
 };
 
 // The lane's values, normed and rotated.  LPH lanes to a head, all of them active.
@@ -60,7 +60,7 @@ __device__ __forceinline__ void norm_rotate(float y[8], const RopeArgs& a, const
 #pragma unroll
     for (int m = LPH / 2; m; m /= 2) t = t + __shfl_xor(t, m, LPH);
     const float r = 1.0f / sqrtf(t * (1.0f / D) + a.eps);
-    const u32x4 wv = load8(w + 8 * lane, a.vec);
+    const u32x4 wv = load8(w + 8 * lane);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       y[i] = (y[i] * r) * to_f32<BF16>((uint16_t)(wv[i / 2] >> (16 * (i & 1))));
@@ -144,7 +144,7 @@ __device__ __forceinline__ void qk_part(const RopeArgs& a, int block) {
   const int kh = h - a.q_heads;
   const uint16_t* src = is_q ? a.q + t * a.q_token + h * a.q_head : a.k + t * a.k_token + kh * a.k_head;
   uint16_t half8[8];
-  unpack8(load8(src + 8 * lane, a.vec), half8);
+  unpack8(load8(src + 8 * lane), half8);
   float y[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) y[i] = to_f32<BF16>(half8[i]);
@@ -211,7 +211,7 @@ __device__ __forceinline__ void value_part(const RopeArgs& a, int block) {
   for (int c = threadIdx.x / LPH; c < n; c += kThreads / LPH) {
     const uint16_t* src = a.v + (t0 + c) * a.v_token + kh * a.v_head;
     uint16_t half8[8];
-    unpack8(load8(src + 8 * lane, a.vec), half8);
+    unpack8(load8(src + 8 * lane), half8);
     float y[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] = to_f32<BF16>(half8[i]);
@@ -317,7 +317,6 @@ __global__ __launch_bounds__(kThreads) void kv4_read_kernel(const ReadArgs a) {
   *reinterpret_cast<u32x4*>(a.v + (int64_t)unit * D + 8 * lane) = rv;
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 int log2_of(int x) { return __builtin_ctz((unsigned)x); }
 
 template <template <int, bool> class K, class A>
@@ -372,8 +371,6 @@ hipError_t launch_rope(const w4a16_rope& t, const w4a16_kv4* kv, const int32_t* 
   a.eps = t.eps;
   a.interleaved = (t.flags & W4A16_KV4_INTERLEAVED) != 0;
   const int D = t.head_dim;
-  int64_t strides = t.q_token | t.q_head | t.k_token | t.k_head;
-  bool vec = aligned16(t.q) && aligned16(t.k) && aligned16(t.q_weight) && aligned16(t.k_weight);
   a.group_lanes = 1;
   const int per_block = kThreads / (D / 8);
   a.qk_blocks = (int)((t.tokens * (t.q_heads + t.kv_heads) + per_block - 1) / per_block);
@@ -382,8 +379,6 @@ hipError_t launch_rope(const w4a16_rope& t, const w4a16_kv4* kv, const int32_t* 
     a.v = static_cast<const uint16_t*>(t.v);
     a.v_token = t.v_token;
     a.v_head = t.v_head;
-    strides |= t.v_token | t.v_head;
-    vec = vec && aligned16(t.v);
     a.pool = kv->pool;
     a.table = kv->table;
     a.rows = rows;
@@ -398,7 +393,6 @@ hipError_t launch_rope(const w4a16_rope& t, const w4a16_kv4* kv, const int32_t* 
     a.chunk = t.tokens * t.kv_heads < 32 * 512 ? 8 : kChunk;
     a.value_blocks = (int)((t.tokens + a.chunk - 1) / a.chunk * t.kv_heads);
   }
-  a.vec = vec && strides % 8 == 0;
   const unsigned blocks = (unsigned)a.qk_blocks + (unsigned)a.value_blocks;
   return by_type<GoRope>(D, t.flags & W4A16_KV4_BF16, a, blocks, st);
 }

@@ -5,42 +5,75 @@
 namespace w4a16 {
 namespace {
 
-// Joins the splits of one query row: D / 4 lanes to a split, a workgroup takes
-// 1024 / D splits at a time.  Bounded by the launch and two dependent reads where
-// rows are few, by memory where they are many.
-template <int D>
+// Most splits of a call, and the most that one group of lanes joins by itself.
+constexpr int kMaxSplits = 256, kFewSplits = 8;
+
+// Joins the splits of a query row; D / 4 lanes to a split, 16 bytes to a lane.
+// kMany: a workgroup takes one row and 1024 / D splits at a time, its weights worked
+// out once and kept in LDS (64 heads, 43 splits: 13.7 us when every lane went
+// through the maxima by itself, 4.6 so); else each group of lanes takes a row of
+// its own.  Bounded by the launch and two dependent reads where rows are few, by
+// memory where they are many.
+template <int D, bool kMany>
 __global__ __launch_bounds__(kAttnThreads) void kv4_join_kernel(const AttnArgs a, int tile_rows,
                                                                 int max_rows) {
-  constexpr int kLanes = D / 4, kAtOnce = kAttnThreads / kLanes;
-  __shared__ f32x4 sum[kAtOnce][kLanes];
-  __shared__ float den[kAtOnce];
+  constexpr int kLanes = D / 4, kGroups = kAttnThreads / kLanes;
+  __shared__ f32x4 sum[kMany ? kGroups : 1][kLanes];
+  __shared__ float weight[kMany ? kMaxSplits : 1], most[4], den[4];
+  const int at = threadIdx.x % kLanes, o = threadIdx.x / kLanes;
+  // rows of a sequence and kv head: rows 0 .. max_rows - 1
   uint32_t id = blockIdx.x;
   const int h = id % a.heads;
   id /= a.heads;
-  const int r = id % max_rows, b = id / max_rows;
+  const int per = kMany ? 1 : kGroups, chunks = (max_rows + per - 1) / per;
+  const int r = (int)(id % chunks) * per + (kMany ? 0 : o), b = id / chunks;
   const AttnSpan s = attn_span(a, b, r / tile_rows * tile_rows, tile_rows);
-  if (r >= s.nq * a.per_kv) return;
+  if (r >= min(max_rows, s.nq * a.per_kv)) return;
   const int i = r / a.per_kv;
   const int64_t qrow = (int64_t)(s.q0 + i) * a.q_heads + h * a.per_kv + (r - i * a.per_kv);
-  const int at = threadIdx.x % kLanes, o = threadIdx.x / kLanes;
-  float m = kNoScore;
-  for (int k = 0; k < s.active; ++k) m = fmaxf(m, part_ml(a, k, qrow, D)[0]);
   f32x4 v = {0, 0, 0, 0};
-  float l = 0.0f;
-  for (int k = o; k < s.active; k += kAtOnce) {
-    const float* ml = part_ml(a, k, qrow, D);
-    const float w = exp2f(ml[0] - m);
-    l += ml[1] * w;
-    v += *reinterpret_cast<const f32x4*>(part_values(a, k, qrow, D) + 4 * at) * w;
-  }
-  sum[o][at] = v;
-  if (at == 0) den[o] = l;
-  __syncthreads();
-  if (o) return;
+  float m = kNoScore, l = 0.0f;
+  if constexpr (kMany) {
+    const int k = threadIdx.x, lane = k & 63, wave = k >> 6;
+    float2 ml = {kNoScore, 0.0f};
+    if (k < s.active) ml = *reinterpret_cast<const float2*>(part_ml(a, k, qrow, D));
+    m = ml.x;
 #pragma unroll
-  for (int k = 1; k < kAtOnce; ++k) {
-    v += sum[k][at];
-    l += den[k];
+    for (int d = 32; d; d /= 2) m = fmaxf(m, __shfl_xor(m, d));
+    if (lane == 0) most[wave] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+    const float w = exp2f(ml.x - m);
+    l = ml.y * w;
+#pragma unroll
+    for (int d = 32; d; d /= 2) l += __shfl_xor(l, d);
+    weight[k] = w;
+    if (lane == 0) den[wave] = l;
+    __syncthreads();
+    l = (den[0] + den[1]) + (den[2] + den[3]);
+#pragma unroll 4
+    for (int j = o; j < s.active; j += kGroups)
+      v += *reinterpret_cast<const f32x4*>(part_values(a, j, qrow, D) + 4 * at) * weight[j];
+    sum[o][at] = v;
+    __syncthreads();
+    if (o) return;
+#pragma unroll
+    for (int j = 1; j < kGroups; ++j) v += sum[j][at];
+  } else {
+    float2 ml[kFewSplits];
+#pragma unroll
+    for (int k = 0; k < kFewSplits; ++k) {
+      ml[k] = {kNoScore, 0.0f};
+      if (k < s.active) ml[k] = *reinterpret_cast<const float2*>(part_ml(a, k, qrow, D));
+      m = fmaxf(m, ml[k].x);
+    }
+#pragma unroll
+    for (int k = 0; k < kFewSplits; ++k) {
+      if (k >= s.active) break;
+      const float w = exp2f(ml[k].x - m);
+      l += ml[k].y * w;
+      v += *reinterpret_cast<const f32x4*>(part_values(a, k, qrow, D) + 4 * at) * w;
+    }
   }
   const bool any = l > 0.0f || l != l;
   const float inv = any ? 1.0f / l : 0.0f;
@@ -49,6 +82,19 @@ __global__ __launch_bounds__(kAttnThreads) void kv4_join_kernel(const AttnArgs a
   for (int j = 0; j < 4; ++j) x[j] = any ? v[j] * inv : 0.0f;
   store4(a.out + qrow * D + 4 * at, x, a.bf16);
   if (a.lse && at == 0) a.lse[qrow] = lse_of(m, l);
+}
+
+template <int D>
+void launch_join(const AttnArgs& a, int tile_rows, int max_rows, hipStream_t st) {
+  if (a.splits > kFewSplits) {
+    kv4_join_kernel<D, true><<<dim3((unsigned)a.heads * max_rows * a.batch), kAttnThreads, 0, st>>>(
+        a, tile_rows, max_rows);
+  } else {
+    constexpr int kGroups = kAttnThreads / (D / 4);
+    kv4_join_kernel<D, false>
+        <<<dim3((unsigned)a.heads * ((max_rows + kGroups - 1) / kGroups) * a.batch), kAttnThreads, 0,
+           st>>>(a, tile_rows, max_rows);
+  }
 }
 
 }  // namespace
@@ -67,10 +113,14 @@ Kv4Plan kv4_attention_plan(const w4a16_kv4& kv, const w4a16_kv4_query& q) {
   // enough workgroups for every CU to hold a few, and for rows of unlike lengths to
   // even out; a split has at least four blocks a wave
   const int64_t units = q.batch * kv.heads * p.tiles, least = p.rows_form ? 8 : 16;
-  int64_t want = (1024 + units - 1) / units;
+  #ifndef KV4_TARGET
+#define KV4_TARGET 1024
+#endif
+  int64_t want = ((p.rows_form ? 512 : KV4_TARGET) + units - 1) / units;
   const int64_t most = (blocks + least - 1) / least;
   if (want > most) want = most;
   if (want < 1) want = 1;
+  if (want > kMaxSplits) want = kMaxSplits;
   p.chunk = (int)((blocks + want - 1) / want);
   if (!p.rows_form) p.chunk = (p.chunk + 3) / 4 * 4;
   p.splits = (int)((blocks + p.chunk - 1) / p.chunk);
@@ -111,7 +161,6 @@ hipError_t launch_kv4_attention(const Kv4Attn& c, hipStream_t st) {
   a.scale_log2 = q.scale * 1.4426950408889634f;
   a.causal = (q.flags & W4A16_KV4_CAUSAL) != 0;
   a.bf16 = (q.flags & W4A16_KV4_BF16) != 0;
-  a.vec = (reinterpret_cast<uintptr_t>(q.q) & 15) == 0 && (q.q_token | q.q_head) % 8 == 0;
   const int D = kv.head_dim, NG = D / kv.group_size;
   const hipError_t e = c.rows_form && D == 256 ? launch_attention_rows256(a, NG, st)
                        : c.rows_form ? launch_attention_rows(a, D, NG, st)
@@ -120,11 +169,10 @@ hipError_t launch_kv4_attention(const Kv4Attn& c, hipStream_t st) {
   if (e != hipSuccess || c.splits == 1) return e;
   const int tile_rows = c.rows_form ? 64 * c.cols : 16 * c.cols;
   const int max_rows = (int)q.max_q * a.per_kv;
-  const dim3 grid((unsigned)a.heads * max_rows * a.batch);
   switch (D) {
-    case 64: kv4_join_kernel<64><<<grid, kAttnThreads, 0, st>>>(a, tile_rows, max_rows); break;
-    case 128: kv4_join_kernel<128><<<grid, kAttnThreads, 0, st>>>(a, tile_rows, max_rows); break;
-    default: kv4_join_kernel<256><<<grid, kAttnThreads, 0, st>>>(a, tile_rows, max_rows); break;
+    case 64: launch_join<64>(a, tile_rows, max_rows, st); break;
+    case 128: launch_join<128>(a, tile_rows, max_rows, st); break;
+    default: launch_join<256>(a, tile_rows, max_rows, st); break;
   }
   return hipGetLastError();
 }

@@ -53,7 +53,7 @@ struct AttnArgs {
   int heads, q_heads, per_kv, batch, tokens;
   int tiles, splits, chunk, window;
   float scale_log2;   // scale * log2(e)
-  bool causal, bf16, vec;
+  bool causal, bf16;
 };
 
 // What a row tile (rows r0 .. r0 + rows - 1 of sequence b and one kv head; row r is
@@ -136,37 +136,41 @@ struct Stage {
   static constexpr int kGroups = 512 * kCodeLoads;        // first group word
   static constexpr int kWords = kGroups + 64 * NG;
 
-  // Word offsets of a lane's first key load, value load and group load in a block.
-  int key, value, group;
+  // Byte offsets of a lane's first key load, value load and group load in a block.
+  uint32_t key, value, group;
   __device__ __forceinline__ Stage(int P, int lane) {
     const int c = lane & 15, g = lane >> 4;
     if constexpr (D == 64) {
       const int j = lane >> 5, cc = (lane & 31) >> 1;     // both tiles in one load
-      key = (8 * (cc >> 2) + 4 * j + (cc & 3)) * (D / 8) + 4 * (lane & 1);
+      key = 4 * ((8 * (cc >> 2) + 4 * j + (cc & 3)) * (D / 8) + 4 * (lane & 1));
     } else {
-      key = (8 * (c >> 2) + (c & 3)) * (D / 8) + g * (D / 32);
+      key = 4 * ((8 * (c >> 2) + (c & 3)) * (D / 8) + g * (D / 32));
     }
-    value = P * (D / 8 + NG) + g * D + 4 * c;
-    group = lane < 32 ? P * (D / 8) + lane : P * (D / 4 + NG) + lane - 32;
+    value = 4 * (P * (D / 8 + NG) + g * D + 4 * c);
+    group = 4 * (lane < 32 ? P * (D / 8) + lane : P * (D / 4 + NG) + lane - 32);
   }
-  // Load q of kLoads of the 32 tokens from t0 on of block `blk`.
-  __device__ __forceinline__ void load(int q, const uint32_t* blk, int P, int t0,
+  // Load q of kLoads of the 32 tokens from t0 on of block `blk` (both the wave's).
+  __device__ __forceinline__ void load(int q, const char* blk, int P, int t0,
                                        uint32_t* lds) const {
-    const uint32_t* from;
-    if (q < kCodeLoads) {
+    if (q < 2 * kCodeLoads) {
+      const char* from = blk + (uint32_t)t0 * (D / 2);   // the wave's part of the address
       const int j = D == 256 ? q >> 1 : q, half = D == 256 ? q & 1 : 0;
-      from = blk + t0 * (D / 8) + key + j * (D / 2) + 4 * half;
-    } else if (q < 2 * kCodeLoads) {
-      from = blk + t0 * (D / 8) + value + 64 * (q - kCodeLoads);
+      if (q < kCodeLoads)
+        from += 4 * (j * (D / 2) + 4 * half);
+      else
+        from += 4 * 64 * (q - kCodeLoads);
+      uint32_t at = q < kCodeLoads ? key : value;
+      asm("" : "+s"(from), "+v"(at));   // (so that the load takes both as they are)
+      __builtin_amdgcn_global_load_lds((const glb_dword*)(from + at),
+                                       (lds_dword*)(lds + 256 * q), 16, 0, 0);
     } else {
-      from = blk + t0 + group + (q - 2 * kCodeLoads) * P;
+      const int n = q - 2 * kCodeLoads;
+      const char* from = blk + (uint32_t)(t0 + n * P) * 4;
+      uint32_t at = group;
+      asm("" : "+s"(from), "+v"(at));
+      __builtin_amdgcn_global_load_lds((const glb_dword*)(from + at),
+                                       (lds_dword*)(lds + kGroups + 64 * n), 4, 0, 0);
     }
-    lds_dword* to = (lds_dword*)(lds + (q < 2 * kCodeLoads ? 256 * q
-                                                           : kGroups + 64 * (q - 2 * kCodeLoads)));
-    if (q < 2 * kCodeLoads)
-      __builtin_amdgcn_global_load_lds((const glb_dword*)from, to, 16, 0, 0);
-    else
-      __builtin_amdgcn_global_load_lds((const glb_dword*)from, to, 4, 0, 0);
   }
 
   // What a lane reads back: the words of key tile j, four value words, the eight
@@ -237,7 +241,8 @@ struct AttnWave {
     mg = make_magic();
   }
 
-  // Row `r` of the lane; rows past the tile's queries see nothing.
+  // Row `r` of the lane, as it lies in memory; rows past the tile's queries see
+  // nothing.
   __device__ __forceinline__ void load_row(const AttnArgs& a, const AttnSpan& s, int h, int r,
                                            int c, int lane) {
     const int i = r / a.per_kv, hh = r - i * a.per_kv, g = lane >> 4;
@@ -247,41 +252,54 @@ struct AttnWave {
     see_lo[c] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
     const uint16_t* src = a.q + (int64_t)(s.q0 + (there ? i : 0)) * a.q_token +
                           (int64_t)(h * a.per_kv + (there ? hh : 0)) * a.q_head;
-    u32x4 x[kSteps];
-    float most = 0.0f;
-    auto value = [&](int k, int j) {
-      const uint16_t u = (uint16_t)(x[k][j / 2] >> (16 * (j & 1)));
-      return a.bf16 ? to_f32<true>(u) : to_f32<false>(u);
-    };
-#pragma unroll
-    for (int k = 0; k < kSteps; ++k) {
-      x[k] = u32x4{0, 0, 0, 0};
-      if (there) x[k] = load8(src + 32 * k + 8 * g, a.vec);
-    }
 #pragma unroll
     for (int k = 0; k < kSteps; ++k)
+      q[c][k] = __builtin_bit_cast(f16x8, load8(src + 32 * k + 8 * g));
+  }
+  // The rows as the first product takes them: 2^e brings a row's largest value into
+  // [2^14, 2^15).
+  template <bool BF16>
+  __device__ __forceinline__ void convert(float scale_log2) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(value(k, j)));
-    // (converted anew below: half the registers)
+    for (int c = 0; c < C; ++c) {
+      u32x4 x[kSteps];
+      float most = 0.0f;
 #pragma unroll
-    for (int k = 0; k < kSteps; ++k) asm volatile("" : "+v"(x[k]));
-    most = max_rows(most);
-    // 2^e brings the largest value into [2^14, 2^15)
-    int e = 0;
-    if (most > 0.0f && most < __builtin_inff()) e = 15 - (__builtin_amdgcn_frexp_expf(most));
+      for (int k = 0; k < kSteps; ++k) {
+        x[k] = __builtin_bit_cast(u32x4, q[c][k]);
 #pragma unroll
-    for (int n = 0; n < NG; ++n) Q[c][n] = 0.0f;
-#pragma unroll
-    for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float y = ldexpf(value(k, j), e);
-        Q[c][k / (kSteps / NG)] += y;
-        q[c][k][j] = (f16)(j & 2 ? y * 0.0625f : y);
+        for (int j = 0; j < 8; ++j)
+          most = fmaxf(most, fabsf(to_f32<BF16>((uint16_t)(x[k][j / 2] >> (16 * (j & 1))))));
       }
+      // (converted anew below: half the registers)
 #pragma unroll
-    for (int n = 0; n < NG; ++n) Q[c][n] = sum_rows(Q[c][n]) * 0x1p-24f;
-    fac[c] = ldexpf(a.scale_log2, 24 - e);
+      for (int k = 0; k < kSteps; ++k) asm volatile("" : "+v"(x[k]));
+      most = max_rows(most);
+      int e = 0;
+      if (most > 0.0f && most < __builtin_inff()) e = 15 - __builtin_amdgcn_frexp_expf(most);
+      // (a subnormal bf16 needs more than fp32's largest power of two: it stays small)
+      e = min(e, 127);
+      const float up = ldexpf(1.0f, e), up16 = ldexpf(1.0f, e - 4);
+#pragma unroll
+      for (int n = 0; n < NG; ++n) Q[c][n] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float y = to_f32<BF16>((uint16_t)(x[k][j / 2] >> (16 * (j & 1))));
+          Q[c][k / (kSteps / NG)] = fmaf(y, up, Q[c][k / (kSteps / NG)]);
+          q[c][k][j] = (f16)(y * (j & 2 ? up16 : up));
+        }
+#pragma unroll
+      for (int n = 0; n < NG; ++n) Q[c][n] = sum_rows(Q[c][n]) * 0x1p-24f;
+      fac[c] = ldexpf(scale_log2, 24 - e);
+    }
+  }
+  __device__ __forceinline__ void convert(const AttnArgs& a) {
+    if (a.bf16)
+      convert<true>(a.scale_log2);
+    else
+      convert<false>(a.scale_log2);
   }
 
   // 32 tokens from t on.  `mask`: some of them are hidden from some row.
@@ -499,26 +517,31 @@ struct PageOf {
 };
 
 // Buffers of 32 tokens a wave (or, rows form, of 64 a workgroup) that are filled in
-// turn.  Three, so that two are on their way while one is worked on; two for heads
-// of 256, where three leave a CU one workgroup.
-template <int D>
-constexpr int kStages = D == 256 ? 2 : 3;
+// turn: one on its way while one is worked on.  A third one costs more waves on a CU
+// than it brings (220 MB of cache, 46 sequences: 81 us with three, 67 with two).
+#ifndef KV4_S
+#define KV4_S 2
+#endif
+constexpr int kStages = KV4_S;
 
 // kRows false: the four waves share 16 * C rows and take blocks of 32 tokens in turn,
 // each through buffers of its own; true: each has 16 * C rows of its own, and all
 // go through the workgroup's blocks together, 64 tokens at a time.  Grid: kv head
 // fastest (an XCD then keeps to few heads and finds their codes in its L2), then
-// split, sequence, and the row tiles from the last, which sees the most tokens, to
-// the first.
+// sequence, split, and the row tiles from the last, which sees the most tokens, to
+// the first.  (Splits before sequences put the empty splits of short sequences on
+// the same CUs: 46 sequences of 1 to 8192 tokens in 4 splits 85 us, in 3 65.)
 // Waves per SIMD that the registers allow without spilling.  Nothing may spill: the
 // loop's counted waits take every load for one of its own.
 template <int D, int NG, int C>
-constexpr int kWaves = C * (D + 32 * (NG - 1)) <= 320 ? 2 : 1;
+constexpr int kWaves = C == 1 && D + 32 * NG <= 160   ? 4
+                       : C == 1 && D + 32 * NG <= 192 ? 3
+                       : C * (D + 32 * (NG - 1)) <= 320 ? 2 : 1;
 
 template <int D, int NG, int C, bool kRows>
 __global__ __launch_bounds__(kAttnThreads, (kWaves<D, NG, C>)) void kv4_attention_kernel(const AttnArgs a) {
   typedef Stage<D, NG> S;
-  constexpr int kTiles = D / 16, kS = kStages<D>;
+  constexpr int kTiles = D / 16, kS = kStages;
   constexpr int kRing = kRows ? kS * 2 * S::kWords : 4 * kS * S::kWords;
   // the four waves' results (rows 4 floats apart beyond D: the four groups of lanes
   // use different banks), then their maxima and denominators
@@ -528,9 +551,9 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<D, NG, C>)) void kv4_attentio
   uint32_t id = blockIdx.x;
   const int h = id % a.heads;
   id /= a.heads;
-  const int split = id % a.splits;
-  id /= a.splits;
-  const int b = id % a.batch, tile = a.tiles - 1 - (int)(id / a.batch);
+  const int b = id % a.batch;
+  id /= a.batch;
+  const int split = id % a.splits, tile = a.tiles - 1 - (int)(id / a.splits);
   const int rows = kRows ? 64 * C : 16 * C;
   const int r0 = tile * rows;
   const AttnSpan s = attn_span(a, b, r0, rows);
@@ -539,8 +562,8 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<D, NG, C>)) void kv4_attentio
   if (a.splits > 1 && split >= s.active) return;
   const int w0 = kRows ? r0 + wave * 16 * C : r0;   // the wave's first row
 
+  // queries first, then the first blocks; the queries are worked on meanwhile
   AttnWave<D, NG, C> w;
-  w.start();
 #pragma unroll
   for (int c = 0; c < C; ++c) w.load_row(a, s, h, w0 + 16 * c + (lane & 15), c, lane);
   // (rows past the last query see nothing, and need no mask to be ignored)
@@ -551,6 +574,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<D, NG, C>)) void kv4_attentio
   w.any_lo = a.window > 0 ? min(max(0, p0 - a.window + 1), w.any_hi) : 0;
   w.all_lo = a.window > 0 ? max(0, p1 - a.window + 1) : 0;
   if (w0 >= R) w.any_hi = 0;
+  w.start();
   {
     // the split's blocks
     const int first = s.first + split * a.chunk;
@@ -561,8 +585,10 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<D, NG, C>)) void kv4_attentio
     const PageOf page{(const const_dword*)(a.table + (int64_t)max(s.row, 0) * a.max_pages),
                       a.page_shift, a.pages};
     const S stage(P, lane);
-    auto block = [&](int pg, int kb) {   // (a missing page's loads go to page 0, unused)
-      return a.pool + ((int64_t)max(pg, 0) * a.heads + h) * words;
+    const char* const head = reinterpret_cast<const char*>(a.pool) + (int64_t)h * words * 4;
+    const uint32_t page_bytes = (uint32_t)a.heads * words * 4;   // (checked to fit by the host)
+    auto block = [&](int pg) {   // (a missing page's loads go to page 0, unused)
+      return head + (uint64_t)(uint32_t)max(pg, 0) * page_bytes;
     };
     if constexpr (kRows) {
       // wave w makes loads w, w + 4, ... of a pair of blocks; the last again where
@@ -574,7 +600,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<D, NG, C>)) void kv4_attentio
         const int pg0 = page(kb), pg1 = page(k1);
         there = (there & ~(3u << (2 * slot))) |
                 ((pg0 >= 0 ? 1u : 0u) | (pg1 >= 0 && kb + 1 < end ? 2u : 0u)) << (2 * slot);
-        const uint32_t *b0 = block(pg0, kb), *b1 = block(pg1, k1);
+        const char *b0 = block(pg0), *b1 = block(pg1);
         uint32_t* to = lds + slot * 2 * S::kWords;
 #pragma unroll
         for (int i = 0; i < kPair; ++i)
@@ -586,6 +612,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<D, NG, C>)) void kv4_attentio
 #pragma unroll
       for (int i = 0; i < kS - 1; ++i)
         if (first + 2 * i < end) fill(i, first + 2 * i);
+      w.convert(a);
       int slot = 0;
       for (int kb = first; kb < end; kb += 2) {
         // this pair is there, by every wave's loads, and the last one read by all
@@ -604,25 +631,27 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<D, NG, C>)) void kv4_attentio
     } else {
       uint32_t* mine = lds + wave * kS * S::kWords;
       uint32_t there = 0;
-      auto fill = [&](int slot, int kb) {
-        const int pg = page(kb);
+      int next = first + wave, pg = page(min(next, max(end - 1, 0)));   // the next to fill
+      auto fill = [&](int slot) {
         there = (there & ~(1u << slot)) | (pg >= 0 ? 1u : 0u) << slot;
-        const uint32_t* from = block(pg, kb);
+        const char* from = block(pg);
 #pragma unroll
         for (int i = 0; i < S::kLoads; ++i)
-          stage.load(i, from, P, (kb << 5) & (P - 1), mine + slot * S::kWords);
+          stage.load(i, from, P, (next << 5) & (P - 1), mine + slot * S::kWords);
+        next += 4;
+        pg = page(min(next, end - 1));   // (asked for a block ahead of its use)
       };
 #pragma unroll
       for (int i = 0; i < kS - 1; ++i)
-        if (first + wave + 4 * i < end) fill(i, first + wave + 4 * i);
+        if (next < end) fill(i);
+      w.convert(a);
       int slot = 0;
       for (int kb = first + wave; kb < end; kb += 4) {
         const int last = slot == 0 ? kS - 1 : slot - 1;
-        const int ahead = kb + 4 * (kS - 1);
-        if (ahead < end) {
+        if (next < end) {
           // (what was read of this buffer has been used: its last values fed products)
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-          fill(last, ahead);
+          fill(last);
           wait_loads<(kS - 1) * S::kLoads>();
         } else if (kS == 3 && kb + 4 < end) {
           wait_loads<S::kLoads>();

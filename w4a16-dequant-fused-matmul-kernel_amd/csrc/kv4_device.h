@@ -60,13 +60,11 @@ __device__ __forceinline__ uint16_t from_f32(float x) {
   return as_u16((f16)x);
 }
 
-// Eight consecutive values; `vec`: the address is 16-byte aligned.
-__device__ __forceinline__ u32x4 load8(const uint16_t* p, bool vec) {
-  if (vec) return *reinterpret_cast<const u32x4*>(p);
-  u32x4 r;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) r[i] = (uint32_t)p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
-  return r;
+// Eight consecutive values, at any element's address (a 16-byte load needs no more
+// than its elements' alignment).
+__device__ __forceinline__ u32x4 load8(const uint16_t* p) {
+  typedef u32x4 loose __attribute__((aligned(2)));
+  return *reinterpret_cast<const loose*>(p);
 }
 
 // Block of a page: -1 where the table has none.  `row`, `at` are checked here, so

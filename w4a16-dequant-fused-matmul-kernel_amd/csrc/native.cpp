@@ -1,6 +1,6 @@
-// _native: the automatic GEMM call as one C function of the CPython API, for the
-// ordinary call (plain strided HIP tensors on the current device, zeros already
-// checked, autotuning off).  Anything else -- wrong types, shapes, layouts or
+// _native: the automatic GEMM call, and those on the 4-bit cache that a decode step
+// makes, as C functions of the CPython API, for the ordinary call (plain strided HIP
+// tensors on the current device, zeros already checked, autotuning off).  Anything else -- wrong types, shapes, layouts or
 // devices, tensor subclasses, functorch wrappers, dispatch modes, an unchecked
 // zeros tensor, an empty result -- returns None, and the caller's Python path
 // checks, raises or computes as it always has.
@@ -24,6 +24,9 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
+#include <cmath>
+
 #include "../../include/w4a16.h"
 
 #ifndef W4A16_NATIVE_HASH
@@ -34,6 +37,15 @@ namespace {
 
 decltype(&w4a16_gemm_f16_auto) g_gemm = nullptr;
 decltype(&w4a16_gemm_workspace_bytes) g_workspace = nullptr;
+decltype(&w4a16_qk_norm_rope) g_rope = nullptr;
+decltype(&w4a16_kv4_append) g_append = nullptr;
+decltype(&w4a16_kv4_read) g_read = nullptr;
+decltype(&w4a16_kv4_attention) g_attention = nullptr;
+decltype(&w4a16_kv4_attention_workspace_bytes) g_attention_workspace = nullptr;
+decltype(&w4a16_kv4_fork) g_fork = nullptr;
+decltype(&w4a16_kv4_fork_workspace_bytes) g_fork_workspace = nullptr;
+decltype(&w4a16_kv4_free) g_free = nullptr;
+decltype(&w4a16_kv4_extend) g_extend = nullptr;
 PyObject* g_zeros_key = nullptr;   // interned attribute name of the zeros check
 
 constexpr int64_t kGroupMultiple = 32;
@@ -197,6 +209,305 @@ PyObject* gemm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- the 4-bit cache (kv4.py) ----------------------------------------------------
+// Each takes what its Python function takes, in order, and returns its result, or
+// None where the Python function has to check, raise or compute.
+
+// A tensor argument (or None, where that may be): false sends the call to Python.
+bool tensor(PyObject* o, const at::Tensor** t, bool may_be_none = false) {
+  if (may_be_none && o == Py_None) return true;
+  return plain(o, t);
+}
+bool integer(PyObject* o, int64_t* v) {
+  if (!PyLong_CheckExact(o)) return false;
+  *v = PyLong_AsLongLong(o);
+  if (*v == -1 && PyErr_Occurred()) {
+    PyErr_Clear();
+    return false;
+  }
+  return true;
+}
+bool ints(const at::Tensor& t, c10::Device dev, int64_t dim) {
+  return t.scalar_type() == at::kInt && t.dim() == dim && t.device() == dev && t.is_contiguous();
+}
+bool list_of(const at::Tensor& t, c10::Device dev, int64_t n) {
+  return ints(t, dev, 1) && t.size(0) == n;
+}
+int32_t* int_ptr(const at::Tensor* t) { return t ? static_cast<int32_t*>(t->data_ptr()) : nullptr; }
+
+// One layer's pool and its table (head_dim, group_size given).
+bool cache(const at::Tensor& pool, const at::Tensor& table, int64_t D, int64_t G, w4a16_kv4* kv) {
+  const auto dev = pool.device();
+  if (!ints(pool, dev, 3) || !ints(table, dev, 2)) return false;
+  if ((D != 64 && D != 128 && D != 256) || G < 32 || (D != G && D != 2 * G && D != 4 * G))
+    return false;
+  const int64_t token = D / 4 + 2 * (D / G), P = pool.size(2) / token;
+  if (P * token != pool.size(2) || P < 32 || P > 256 || (P & (P - 1))) return false;
+  *kv = w4a16_kv4{int_ptr(&pool), int_ptr(&table), pool.size(0), table.size(0), table.size(1),
+                  (int32_t)pool.size(1), (int32_t)D, (int32_t)G, (int32_t)P};
+  return true;
+}
+bool heads3(const at::Tensor& t, const at::Tensor& like) {
+  return t.dim() == 3 && t.stride(2) == 1 && t.scalar_type() == like.scalar_type() &&
+         t.device() == like.device() && t.size(0) == like.size(0) && t.size(2) == like.size(2);
+}
+bool here(const at::Tensor& t) { return c10::hip::current_device() == t.device().index(); }
+void* stream_of(const at::Tensor& t) {
+  return c10::hip::getCurrentHIPStream(t.device().index()).stream();
+}
+
+// The arguments that append and the dense call share: q, k, [v], cos, sin, positions,
+// q_weight, k_weight, eps, interleaved.
+bool rope_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor* v, const at::Tensor& cos,
+               const at::Tensor& sin, const at::Tensor& positions, const at::Tensor* wq,
+               const at::Tensor* wk, PyObject* eps, PyObject* interleaved, w4a16_rope* r) {
+  const auto type = q.scalar_type();
+  if (q.dim() != 3 || (type != at::kHalf && type != at::kBFloat16) || !heads3(q, q) ||
+      !heads3(k, q) || (v && (!heads3(*v, q) || v->size(1) != k.size(1))) || !here(q))
+    return false;
+  const auto dev = q.device();
+  const int64_t T = q.size(0), D = q.size(2);
+  for (const at::Tensor* t : {&cos, &sin})
+    if (t->scalar_type() != at::kFloat || t->dim() != 2 || t->device() != dev || !t->is_contiguous())
+      return false;
+  if (cos.sizes() != sin.sizes() || !list_of(positions, dev, T) || !PyFloat_CheckExact(eps) ||
+      !PyBool_Check(interleaved))
+    return false;
+  for (const at::Tensor* w : {wq, wk})
+    if (w && (w->dim() != 1 || w->size(0) != D || w->scalar_type() != type || w->device() != dev ||
+              !w->is_contiguous()))
+      return false;
+  *r = w4a16_rope{};
+  r->q = q.data_ptr();
+  r->k = k.data_ptr();
+  r->q_token = q.stride(0);
+  r->q_head = q.stride(1);
+  r->k_token = k.stride(0);
+  r->k_head = k.stride(1);
+  if (v) {
+    r->v = v->data_ptr();
+    r->v_token = v->stride(0);
+    r->v_head = v->stride(1);
+  }
+  r->cos = static_cast<const float*>(cos.data_ptr());
+  r->sin = static_cast<const float*>(sin.data_ptr());
+  r->token_position = int_ptr(&positions);
+  r->q_weight = wq ? wq->data_ptr() : nullptr;
+  r->k_weight = wk ? wk->data_ptr() : nullptr;
+  r->tokens = T;
+  r->positions = cos.size(0);
+  r->q_heads = (int32_t)q.size(1);
+  r->kv_heads = (int32_t)k.size(1);
+  r->head_dim = (int32_t)D;
+  r->rot_dim = (int32_t)(2 * cos.size(1));
+  r->eps = (float)PyFloat_AS_DOUBLE(eps);
+  r->flags = (type == at::kBFloat16 ? W4A16_KV4_BF16 : 0) |
+             (interleaved == Py_True ? W4A16_KV4_INTERLEAVED : 0);
+  return true;
+}
+
+// qk_norm_rope(q, k, cos, sin, positions, q_weight, k_weight, eps, interleaved)
+PyObject* qk_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *q, *k, *cos, *sin, *pos, *wq = nullptr, *wk = nullptr;
+  w4a16_rope r;
+  if (n != 9 || !g_rope || !tensor(args[0], &q) || !tensor(args[1], &k) || !tensor(args[2], &cos) ||
+      !tensor(args[3], &sin) || !tensor(args[4], &pos) || !tensor(args[5], &wq, true) ||
+      !tensor(args[6], &wk, true) || observed() ||
+      !rope_args(*q, *k, nullptr, *cos, *sin, *pos, wq, wk, args[7], args[8], &r))
+    Py_RETURN_NONE;
+  at::Tensor qo = at::empty(q->sizes(), q->options()), ko = at::empty(k->sizes(), q->options());
+  r.q_out = qo.data_ptr();
+  r.k_out = ko.data_ptr();
+  if (g_rope(&r, stream_of(*q)) != W4A16_OK) Py_RETURN_NONE;
+  PyObject* both = PyTuple_New(2);
+  if (!both) return nullptr;
+  PyTuple_SET_ITEM(both, 0, THPVariable_Wrap(std::move(qo)));
+  PyTuple_SET_ITEM(both, 1, THPVariable_Wrap(std::move(ko)));
+  return both;
+  END_HANDLE_TH_ERRORS
+}
+
+// kv4_append(q, k, v, cos, sin, positions, pool, table, rows, group_size, q_weight,
+//            k_weight, eps, interleaved)
+PyObject* kv4_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *q, *k, *v, *cos, *sin, *pos, *pool, *table, *rows = nullptr, *wq = nullptr,
+                                                               *wk = nullptr;
+  int64_t G;
+  w4a16_rope r;
+  w4a16_kv4 kv;
+  if (n != 14 || !g_append || !tensor(args[0], &q) || !tensor(args[1], &k) || !tensor(args[2], &v) ||
+      !tensor(args[3], &cos) || !tensor(args[4], &sin) || !tensor(args[5], &pos) ||
+      !tensor(args[6], &pool) || !tensor(args[7], &table) || !tensor(args[8], &rows, true) ||
+      !integer(args[9], &G) || !tensor(args[10], &wq, true) || !tensor(args[11], &wk, true) ||
+      observed() || !rope_args(*q, *k, v, *cos, *sin, *pos, wq, wk, args[12], args[13], &r) ||
+      !cache(*pool, *table, q->size(2), G, &kv) || pool->device() != q->device() ||
+      (rows && !list_of(*rows, q->device(), q->size(0))))
+    Py_RETURN_NONE;
+  at::Tensor qo = at::empty(q->sizes(), q->options());
+  r.q_out = qo.data_ptr();
+  if (g_append(&r, &kv, int_ptr(rows), stream_of(*q)) != W4A16_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(qo));
+  END_HANDLE_TH_ERRORS
+}
+
+// kv4_read(pool, table, positions, rows, head_dim, group_size, bf16)
+PyObject* kv4_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *pool, *table, *pos, *rows = nullptr;
+  int64_t D, G;
+  w4a16_kv4 kv;
+  if (n != 7 || !g_read || !tensor(args[0], &pool) || !tensor(args[1], &table) ||
+      !tensor(args[2], &pos) || !tensor(args[3], &rows, true) || !integer(args[4], &D) ||
+      !integer(args[5], &G) || !PyBool_Check(args[6]) || observed() || !here(*pool) ||
+      !cache(*pool, *table, D, G, &kv) || !ints(*pos, pool->device(), 1) ||
+      (rows && !list_of(*rows, pool->device(), pos->size(0))))
+    Py_RETURN_NONE;
+  const int64_t T = pos->size(0);
+  const bool bf16 = args[6] == Py_True;
+  const auto opt = at::TensorOptions().dtype(bf16 ? at::kBFloat16 : at::kHalf).device(pool->device());
+  at::Tensor k = at::empty({T, pool->size(1), D}, opt), v = at::empty({T, pool->size(1), D}, opt);
+  if (g_read(&kv, int_ptr(pos), int_ptr(rows), T, k.data_ptr(), v.data_ptr(),
+             bf16 ? W4A16_KV4_BF16 : 0, stream_of(*pool)) != W4A16_OK)
+    Py_RETURN_NONE;
+  PyObject* both = PyTuple_New(2);
+  if (!both) return nullptr;
+  PyTuple_SET_ITEM(both, 0, THPVariable_Wrap(std::move(k)));
+  PyTuple_SET_ITEM(both, 1, THPVariable_Wrap(std::move(v)));
+  return both;
+  END_HANDLE_TH_ERRORS
+}
+
+// kv4_attention(q, pool, table, lens, q_starts, seqs, max_q | None, max_context |
+//               None, group_size, scale | None, causal, window)
+PyObject* kv4_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *q, *pool, *table, *lens, *starts = nullptr, *seqs = nullptr;
+  int64_t G, window, max_q = -1, max_context = -1;
+  w4a16_kv4 kv;
+  if (n != 12 || !g_attention || !tensor(args[0], &q) || !tensor(args[1], &pool) ||
+      !tensor(args[2], &table) || !tensor(args[3], &lens) || !tensor(args[4], &starts, true) ||
+      !tensor(args[5], &seqs, true) || (args[6] != Py_None && !integer(args[6], &max_q)) ||
+      (args[7] != Py_None && !integer(args[7], &max_context)) || !integer(args[8], &G) ||
+      (args[9] != Py_None && !PyFloat_CheckExact(args[9])) || !PyBool_Check(args[10]) ||
+      !integer(args[11], &window) || observed())
+    Py_RETURN_NONE;
+  const auto type = q->scalar_type();
+  const auto dev = q->device();
+  if (q->dim() != 3 || (type != at::kHalf && type != at::kBFloat16) || q->stride(2) != 1 ||
+      !here(*q) || pool->device() != dev || !cache(*pool, *table, q->size(2), G, &kv) ||
+      !list_of(*lens, dev, table->size(0)))
+    Py_RETURN_NONE;
+  const int64_t T = q->size(0), D = q->size(2), most = kv.max_pages * kv.page_size;
+  int64_t batch = T;
+  if (starts) {
+    if (!ints(*starts, dev, 1) || starts->size(0) < 1) Py_RETURN_NONE;
+    batch = starts->size(0) - 1;
+  }
+  if (seqs ? !list_of(*seqs, dev, batch) : batch > table->size(0)) Py_RETURN_NONE;
+  const double scale = args[9] != Py_None ? PyFloat_AS_DOUBLE(args[9]) : 1.0 / std::sqrt((double)D);
+  if ((args[6] != Py_None && max_q < 0) || (args[7] != Py_None && max_context < 0) || window < 0)
+    Py_RETURN_NONE;
+  w4a16_kv4_query a{};
+  a.q = q->data_ptr();
+  a.q_token = q->stride(0);
+  a.q_head = q->stride(1);
+  a.lens = int_ptr(lens);
+  a.q_starts = int_ptr(starts);
+  a.seqs = int_ptr(seqs);
+  a.tokens = T;
+  a.batch = batch;
+  a.max_q = max_q < 0 ? T : max_q;
+  a.max_context = std::min<int64_t>(max_context < 0 ? most : max_context, INT32_MAX);
+  a.q_heads = (int32_t)q->size(1);
+  a.window = (int32_t)std::min<int64_t>(window, INT32_MAX);
+  a.scale = (float)scale;
+  a.flags = (type == at::kBFloat16 ? W4A16_KV4_BF16 : 0) |
+            (args[10] == Py_True ? W4A16_KV4_CAUSAL : 0);
+  at::Tensor out = at::empty(q->sizes(), q->options()), ws;
+  a.out = out.data_ptr();
+  const size_t bytes = g_attention_workspace(&kv, &a);
+  if (bytes) ws = at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(dev));
+  if (g_attention(&kv, &a, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(*q)) != W4A16_OK)
+    Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+bool book_of(const at::Tensor& table, const at::Tensor& lens, const at::Tensor& refs, int64_t P,
+             w4a16_kv4_book* b) {
+  const auto dev = table.device();
+  if (!here(table) || !ints(table, dev, 2) || !list_of(lens, dev, table.size(0)) ||
+      !ints(refs, dev, 1))
+    return false;
+  *b = w4a16_kv4_book{int_ptr(&table), int_ptr(&lens), int_ptr(&refs), table.size(0),
+                      table.size(1), refs.size(0), (int32_t)P};
+  return true;
+}
+
+// kv4_free(table, lens, refs, seqs): True
+PyObject* kv4_free(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *table, *lens, *refs, *seqs;
+  w4a16_kv4_book b;
+  if (n != 4 || !g_free || !tensor(args[0], &table) || !tensor(args[1], &lens) ||
+      !tensor(args[2], &refs) || !tensor(args[3], &seqs) || observed() ||
+      !book_of(*table, *lens, *refs, 32, &b) || !ints(*seqs, table->device(), 1) ||
+      g_free(&b, int_ptr(seqs), seqs->size(0), stream_of(*table)) != W4A16_OK)
+    Py_RETURN_NONE;
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// kv4_extend(table, lens, refs, seqs, counts, page_size, status): True
+PyObject* kv4_extend(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *table, *lens, *refs, *seqs, *counts, *status;
+  int64_t P;
+  w4a16_kv4_book b;
+  if (n != 7 || !g_extend || !tensor(args[0], &table) || !tensor(args[1], &lens) ||
+      !tensor(args[2], &refs) || !tensor(args[3], &seqs) || !tensor(args[4], &counts) ||
+      !integer(args[5], &P) || !tensor(args[6], &status) || observed() ||
+      !book_of(*table, *lens, *refs, P, &b) || !ints(*seqs, table->device(), 1) ||
+      !list_of(*counts, table->device(), seqs->size(0)) ||
+      !list_of(*status, table->device(), 1) ||
+      g_extend(&b, int_ptr(seqs), int_ptr(counts), seqs->size(0), int_ptr(status),
+               stream_of(*table)) != W4A16_OK)
+    Py_RETURN_NONE;
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// kv4_fork(pool, table, lens, refs, parents, children, page_size, status): True
+PyObject* kv4_fork(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *pool, *table, *lens, *refs, *parents, *children, *status;
+  int64_t P;
+  w4a16_kv4_book b;
+  if (n != 8 || !g_fork || !tensor(args[0], &pool) || !tensor(args[1], &table) ||
+      !tensor(args[2], &lens) || !tensor(args[3], &refs) || !tensor(args[4], &parents) ||
+      !tensor(args[5], &children) || !integer(args[6], &P) || !tensor(args[7], &status) ||
+      observed() || !book_of(*table, *lens, *refs, P, &b))
+    Py_RETURN_NONE;
+  const auto dev = table->device();
+  const int64_t dim = pool->dim();
+  if ((dim != 3 && dim != 4) || !ints(*pool, dev, dim) || pool->size(dim - 3) != refs->size(0) ||
+      !ints(*parents, dev, 1) || !list_of(*children, dev, parents->size(0)) ||
+      !list_of(*status, dev, 1))
+    Py_RETURN_NONE;
+  const int64_t count = parents->size(0);
+  const size_t bytes = g_fork_workspace(count);
+  at::Tensor ws;
+  if (bytes) ws = at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(dev));
+  if (g_fork(int_ptr(pool), dim == 4 ? pool->size(0) : 1, pool->size(dim - 2) * pool->size(dim - 1),
+             &b, int_ptr(parents), int_ptr(children), count, int_ptr(status),
+             bytes ? ws.data_ptr() : nullptr, bytes, stream_of(*pool)) != W4A16_OK)
+    Py_RETURN_NONE;
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
 // init(path of the loaded libw4a16.so, name of the zeros check's attribute)
 PyObject* init(PyObject*, PyObject* args) {
   const char *path, *key;
@@ -213,6 +524,18 @@ PyObject* init(PyObject*, PyObject* args) {
     PyErr_Format(PyExc_ImportError, "%s lacks w4a16_gemm_f16_auto", path);
     return nullptr;
   }
+  // (the loader has checked that every declared symbol is there)
+  g_rope = reinterpret_cast<decltype(g_rope)>(dlsym(lib, "w4a16_qk_norm_rope"));
+  g_append = reinterpret_cast<decltype(g_append)>(dlsym(lib, "w4a16_kv4_append"));
+  g_read = reinterpret_cast<decltype(g_read)>(dlsym(lib, "w4a16_kv4_read"));
+  g_attention_workspace = reinterpret_cast<decltype(g_attention_workspace)>(
+      dlsym(lib, "w4a16_kv4_attention_workspace_bytes"));
+  g_attention = reinterpret_cast<decltype(g_attention)>(dlsym(lib, "w4a16_kv4_attention"));
+  g_fork_workspace = reinterpret_cast<decltype(g_fork_workspace)>(
+      dlsym(lib, "w4a16_kv4_fork_workspace_bytes"));
+  g_fork = reinterpret_cast<decltype(g_fork)>(dlsym(lib, "w4a16_kv4_fork"));
+  g_free = reinterpret_cast<decltype(g_free)>(dlsym(lib, "w4a16_kv4_free"));
+  g_extend = reinterpret_cast<decltype(g_extend)>(dlsym(lib, "w4a16_kv4_extend"));
   g_zeros_key = PyUnicode_InternFromString(key);
   if (!g_zeros_key) return nullptr;
   Py_RETURN_NONE;
@@ -223,6 +546,20 @@ PyObject* build_id(PyObject*, PyObject*) { return PyUnicode_FromString(W4A16_NAT
 PyMethodDef kMethods[] = {
     {"gemm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(gemm)), METH_FASTCALL,
      "The automatic GEMM call, or None where the Python path has to make it."},
+    {"qk_norm_rope", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(qk_norm_rope)), METH_FASTCALL,
+     "kv4.py: qk_norm_rope, or None where the Python path has to make the call."},
+    {"kv4_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(kv4_append)), METH_FASTCALL,
+     "kv4.py: kv4_append, or None where the Python path has to make the call."},
+    {"kv4_read", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(kv4_read)), METH_FASTCALL,
+     "kv4.py: kv4_read, or None where the Python path has to make the call."},
+    {"kv4_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(kv4_attention)), METH_FASTCALL,
+     "kv4.py: kv4_attention, or None where the Python path has to make the call."},
+    {"kv4_free", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(kv4_free)), METH_FASTCALL,
+     "kv4.py: kv4_free, or None where the Python path has to make the call."},
+    {"kv4_extend", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(kv4_extend)), METH_FASTCALL,
+     "kv4.py: kv4_extend, or None where the Python path has to make the call."},
+    {"kv4_fork", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(kv4_fork)), METH_FASTCALL,
+     "kv4.py: kv4_fork, or None where the Python path has to make the call."},
     {"init", init, METH_VARARGS, "Bind the loaded libw4a16.so."},
     {"build_id", build_id, METH_NOARGS, "sha256 of the sources this module was built from."},
     {nullptr, nullptr, 0, nullptr}};

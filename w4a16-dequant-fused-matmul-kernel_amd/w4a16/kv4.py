@@ -30,17 +30,42 @@ from __future__ import annotations
 
 import ctypes
 import math
+import warnings
 
 import torch
 from torch import Tensor
 
 from . import _lib
 from . import _runtime as rt
+from .hip_kernel import _ZKEY
 
 __all__ = ["qk_norm_rope", "kv4_append", "kv4_read", "kv4_attention", "kv4_copy_pages",
            "kv4_extend", "kv4_fork", "kv4_free", "kv4_compact", "kv4_words"]
 
 _TYPES = (torch.float16, torch.bfloat16)
+
+
+class _Native:
+    """The native forms of the calls below (csrc/native.cpp), loaded by the first one.
+    Without a module of these sources and this torch every call is checked and
+    launched from Python instead: the same kernels and results, 8-15 us more host
+    time a call."""
+
+    def __getattr__(self, name):
+        try:
+            mod = _lib.load_native(_ZKEY)
+        except ImportError as e:
+            warnings.warn(f"w4a16: {e}; calls are checked and launched from Python meanwhile "
+                          "(the same kernels, 8-15 us more host time each)", RuntimeWarning,
+                          stacklevel=3)
+            mod = None
+        for f in ("qk_norm_rope", "kv4_append", "kv4_read", "kv4_attention", "kv4_free",
+                  "kv4_extend", "kv4_fork"):
+            setattr(self, f, getattr(mod, f) if mod else lambda *args: None)
+        return self.__dict__[name]
+
+
+_native = _Native()
 
 
 def kv4_words(head_dim: int, group_size: int, page_size: int) -> int:
@@ -160,6 +185,10 @@ def qk_norm_rope(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, positions: Tens
     Returns:
         (queries, keys), computed in fp32 and rounded once.
     """
+    if out is None:
+        both = _native.qk_norm_rope(q, k, cos, sin, positions, q_weight, k_weight, eps, interleaved)
+        if both is not None:
+            return both
     r = _rope(q, k, None, cos, sin, positions, q_weight, k_weight, eps, interleaved)
     qo = _dense(q, q.shape[1], out and out[0], "out[0]")
     ko = _dense(q, k.shape[1], out and out[1], "out[1]")
@@ -181,6 +210,11 @@ def kv4_append(q: Tensor, k: Tensor, v: Tensor, cos: Tensor, sin: Tensor, positi
     page for, is not stored.  No two tokens of a call may have the same place.
     Returns the queries.
     """
+    if out is None:
+        y = _native.kv4_append(q, k, v, cos, sin, positions, pool, table, rows, group_size,
+                               q_weight, k_weight, eps, interleaved)
+        if y is not None:
+            return y
     r = _rope(q, k, v, cos, sin, positions, q_weight, k_weight, eps, interleaved)
     kv = _kv4(pool, table, q.shape[2], group_size)
     assert pool.device == q.device, f"pool must be on {q.device}"
@@ -201,6 +235,11 @@ def kv4_read(pool: Tensor, table: Tensor, positions: Tensor, *, head_dim: int,
              dtype: torch.dtype = torch.float16) -> tuple[Tensor, Tensor]:
     """Stored tokens, (keys, values) [tokens, heads, head_dim]: the inverse of the
     storing in ``kv4_append``.  Zeros for a place that the table does not hold."""
+    if dtype in _TYPES:
+        both = _native.kv4_read(pool, table, positions, rows, head_dim, group_size,
+                                dtype == torch.bfloat16)
+        if both is not None:
+            return both
     kv = _kv4(pool, table, head_dim, group_size)
     assert dtype in _TYPES, f"dtype must be fp16 or bf16, got {dtype}"
     assert positions.dim() == 1, f"positions must be [tokens], got {list(positions.shape)}"
@@ -246,6 +285,11 @@ def kv4_attention(q: Tensor, pool: Tensor, table: Tensor, lens: Tensor, *,
     Returns:
         [tokens, q_heads, head_dim]; zeros (lse -inf) for a token that sees nothing.
     """
+    if out is None and not return_lse:
+        y = _native.kv4_attention(q, pool, table, lens, q_starts, seqs, max_q, max_context,
+                                  group_size, scale, causal, window)
+        if y is not None:
+            return y
     _heads3(q, "q")
     T, Hq, D = q.shape
     dev = q.device
@@ -353,6 +397,9 @@ def kv4_extend(table: Tensor, lens: Tensor, refs: Tensor, seqs: Tensor, counts: 
     ``KV4Cache.NO_PAGES``, ``ROW_FULL`` and ``BAD_ROW``; such a row is unchanged.
     Returned, so that a caller may look when it next waits for the device.
     """
+    if status is not None and _native.kv4_extend(table, lens, refs, seqs, counts, page_size,
+                                                 status):
+        return status
     book = _book(table, lens, refs, page_size)
     dev = table.device
     n = _list(seqs, "seqs", dev)
@@ -370,6 +417,9 @@ def kv4_fork(pool: Tensor, table: Tensor, lens: Tensor, refs: Tensor, parents: T
     """Row ``children[i]`` (empty, named once) becomes a copy of row ``parents[i]``:
     whole pages are shared, a partly filled last page is copied, in every layer, to
     the lowest free one.  Returns the status (see ``kv4_extend``)."""
+    if status is not None and _native.kv4_fork(pool, table, lens, refs, parents, children,
+                                               page_size, status):
+        return status
     layers, pages, words = _pool4(pool)
     book = _book(table, lens, refs, page_size)
     dev = pool.device
@@ -389,6 +439,8 @@ def kv4_fork(pool: Tensor, table: Tensor, lens: Tensor, refs: Tensor, parents: T
 
 def kv4_free(table: Tensor, lens: Tensor, refs: Tensor, seqs: Tensor) -> None:
     """Empty rows ``seqs``; a page that no other row holds is free afterwards."""
+    if _native.kv4_free(table, lens, refs, seqs):
+        return
     book = _book(table, lens, refs, 32)   # (whatever a page holds)
     dev = table.device
     n = _list(seqs, "seqs", dev)

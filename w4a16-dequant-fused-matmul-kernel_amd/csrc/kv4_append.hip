@@ -14,8 +14,14 @@
 // halves -- so a token's results are the same bits whether it comes alone or in a
 // prompt, and can be reproduced by elementwise arithmetic.
 //
-// Queries and keys: D / 8 lanes to a head, eight consecutive values to a lane.
-// A lane's eight key codes are one word of the cache.  Values: a cache word holds
+// Where tokens are many the issue of vector instructions bounds it, not memory: a
+// lane has only eight values of a head, so what does not depend on them is shared.
+//
+// D / 8 lanes to a head, eight consecutive values to a lane.  Queries (and keys that
+// are not stored): a workgroup takes heads of one token and each group of lanes up
+// to four of them together, with one set of cosines, and one square root and
+// quotient for the four, each worked out by a quarter of the lanes.  Stored keys: a
+// group of lanes takes one head; a lane's eight codes are one word of the cache.  Values: a cache word holds
 // eight tokens of one value, so a workgroup quantises a chunk of tokens of one
 // head into LDS and then writes words.  A word whose eight tokens are all in the
 // chunk is stored whole; any other keeps the codes of its other tokens, which
@@ -23,6 +29,8 @@
 // bits (an exclusive or with what it read of them), so the order does not matter.
 #include "kv4_device.h"
 #include "kv4_launch.h"
+
+#include <type_traits>
 
 #pragma clang fp contract(off)
 
@@ -43,63 +51,127 @@ struct RopeArgs {
   int tokens, positions, q_heads, kv_heads, half;   // half: rotated pairs of a head
   int table_rows, max_pages, pages, page_shift;
   int group_lanes, NG;                              // lanes of D / 8 that share a group
-  int chunk, value_blocks, qk_blocks;
+  int chunk, value_blocks;
+  int q_blocks, q_parts, k_blocks, k_parts;         // workgroups, and those of a token
   float eps;
-  bool interleaved, store;
+  bool interleaved, store, four;
 };
 
-// The lane's values, normed and rotated.  LPH lanes to a head, all of them active.
-template <int LPH, bool BF16>
-__device__ __forceinline__ void norm_rotate(float y[8], const RopeArgs& a, const uint16_t* w,
-                                            int pos, int lane) {
-  constexpr int D = 8 * LPH;
-  if (w) {
-    const float t0 = y[0] * y[0] + y[4] * y[4], t1 = y[1] * y[1] + y[5] * y[5];
-    const float t2 = y[2] * y[2] + y[6] * y[6], t3 = y[3] * y[3] + y[7] * y[7];
-    float t = (t0 + t2) + (t1 + t3);
+// v of lane ^ M.  Within 16 lanes by DPP (quad permutations, a mirror of eight lanes
+// and a rotation by eight), which needs no LDS.
+template <int M>
+__device__ __forceinline__ float xor_lane(float v) {
+  auto dpp = [](float x, auto ctrl) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x),
+                                                                 decltype(ctrl)::value, 0xF, 0xF,
+                                                                 false));
+  };
+  if constexpr (M == 1) return dpp(v, std::integral_constant<int, 0xB1>{});
+  if constexpr (M == 2) return dpp(v, std::integral_constant<int, 0x4E>{});
+  if constexpr (M == 4)   // mirrored within eight lanes, then within four
+    return dpp(dpp(v, std::integral_constant<int, 0x141>{}), std::integral_constant<int, 0x1B>{});
+  if constexpr (M == 8) return dpp(v, std::integral_constant<int, 0x128>{});
+  return __shfl_xor(v, M);
+}
+
+// v of lane J of the lane's four.
+template <int J>
+__device__ __forceinline__ float quad_lane(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v),
+                                                               J * 0x55, 0xF, 0xF, false));
+}
+
+// What a lane needs of its token's rotation: y * c + partner * s for each of its
+// values (for values that rotate together, its four pairs' cosines and sines).
+struct Turn {
+  float c[8], s[8];
+  bool inside, turns;   // the tables hold the position; the lane's values rotate
+  int partner;          // lane of the other half
+};
+template <int LPH>
+__device__ __forceinline__ Turn turn_of(const RopeArgs& a, int pos, int lane) {
+  Turn t;
+  t.inside = (uint32_t)pos < (uint32_t)a.positions;
+  const int64_t row = (int64_t)(t.inside ? pos : 0) * a.half;
+  const int hl = a.half >> 3;   // lanes of one half
+  const bool low = lane < hl;
+  t.turns = lane < 2 * hl;
+  t.partner = low ? lane + hl : t.turns ? lane - hl : lane;
+  const int n = a.interleaved ? 4 : 8;
+  const int at = !t.turns ? 0 : a.interleaved ? 4 * lane : 8 * (low ? lane : lane - hl);
 #pragma unroll
-    for (int m = LPH / 2; m; m /= 2) t = t + __shfl_xor(t, m, LPH);
-    const float r = 1.0f / sqrtf(t * (1.0f / D) + a.eps);
-    const u32x4 wv = load8(w + 8 * lane);
+  for (int i = 0; i < 8; i += 4) {
+    f32x4 c = {1, 1, 1, 1}, s = {0, 0, 0, 0};
+    if (i < n && t.turns && a.positions > 0) {
+      typedef f32x4 loose __attribute__((aligned(4)));
+      c = *reinterpret_cast<const loose*>(a.cos + row + at + i);
+      s = *reinterpret_cast<const loose*>(a.sin + row + at + i);
+    }
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      y[i] = (y[i] * r) * to_f32<BF16>((uint16_t)(wv[i / 2] >> (16 * (i & 1))));
+    for (int j = 0; j < 4; ++j) {
+      t.c[i + j] = c[j];
+      t.s[i + j] = low && !a.interleaved ? -s[j] : s[j];
+    }
   }
-  const bool inside = (uint32_t)pos < (uint32_t)a.positions;
-  const float* c = a.cos + (int64_t)(inside ? pos : 0) * a.half;
-  const float* s = a.sin + (int64_t)(inside ? pos : 0) * a.half;
-  const float bad = inside ? 0.0f : __builtin_nanf("");
+  return t;
+}
+
+// Sum of the squares of a head, in every one of its lanes.
+template <int LPH>
+__device__ __forceinline__ float squares(const float y[8]) {
+  const float t0 = y[0] * y[0] + y[4] * y[4], t1 = y[1] * y[1] + y[5] * y[5];
+  const float t2 = y[2] * y[2] + y[6] * y[6], t3 = y[3] * y[3] + y[7] * y[7];
+  float q = (t0 + t2) + (t1 + t3);
+  if constexpr (LPH == 32) q = q + xor_lane<16>(q);
+  if constexpr (LPH >= 16) q = q + xor_lane<8>(q);
+  q = q + xor_lane<4>(q);
+  q = q + xor_lane<2>(q);
+  return q + xor_lane<1>(q);
+}
+template <int LPH>
+__device__ __forceinline__ float root(float squares, float eps) {
+  return 1.0f / sqrtf(squares * (1.0f / (8 * LPH)) + eps);
+}
+
+template <int LPH>
+__device__ __forceinline__ void rotate(float y[8], const RopeArgs& a, const Turn& t) {
   if (a.interleaved) {
-    if (8 * lane < 2 * a.half) {
+    if (t.turns) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float cc = c[4 * lane + i] + bad, ss = s[4 * lane + i] + bad;
         const float p = y[2 * i], q = y[2 * i + 1];
-        y[2 * i] = p * cc - q * ss;
-        y[2 * i + 1] = q * cc + p * ss;
+        y[2 * i] = p * t.c[i] - q * t.s[i];
+        y[2 * i + 1] = q * t.c[i] + p * t.s[i];
       }
     }
-  } else {
-    const int hl = a.half >> 3;   // lanes of one half
-    const bool low = lane < hl, turn = lane < 2 * hl;
-    const int other = low ? lane + hl : turn ? lane - hl : lane;
-    const int at = turn ? 8 * (low ? lane : other) : 0;
+  } else if (a.half == 4 * LPH) {   // the whole head: partners are half a head apart
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float o = __shfl(y[i], other, LPH);
-      const float cc = c[at + i] + bad, ss = s[at + i] + bad;
-      const float r = low ? y[i] * cc - o * ss : y[i] * cc + o * ss;
-      y[i] = turn ? r : y[i];
+      const float o = xor_lane<LPH / 2>(y[i]);
+      y[i] = y[i] * t.c[i] + o * t.s[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float o = __shfl(y[i], t.partner, LPH);
+      const float r = y[i] * t.c[i] + o * t.s[i];
+      y[i] = t.turns ? r : y[i];
     }
   }
-  if (!inside) {   // values that do not rotate as well
+  if (!t.inside) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] += bad;
+    for (int i = 0; i < 8; ++i) y[i] = __builtin_nanf("");
   }
 }
 
-// Codes of a lane's eight values with the group's word; group_lanes lanes to a group.
-__device__ __forceinline__ uint32_t quantise(const float y[8], int group_lanes, uint32_t code[8]) {
+// Codes of a lane's eight values, the i-th at bit `at(i)`, or 8 everywhere where the
+// group has no scale, with the group's word; group_lanes lanes to a group.
+struct Codes {
+  uint32_t code[8], group;
+  bool ok;
+};
+template <int LPH>
+__device__ __forceinline__ Codes quantise(const float y[8], int group_lanes) {
   // (a minimum that keeps NaN: one such value makes its whole group NaN)
   float lo = y[0], hi = y[0];
 #pragma unroll
@@ -107,21 +179,32 @@ __device__ __forceinline__ uint32_t quantise(const float y[8], int group_lanes, 
     lo = __builtin_elementwise_minimum(lo, y[i]);
     hi = __builtin_elementwise_maximum(hi, y[i]);
   }
-  for (int m = 1; m < group_lanes; m *= 2) {
-    lo = __builtin_elementwise_minimum(lo, __shfl_xor(lo, m));
-    hi = __builtin_elementwise_maximum(hi, __shfl_xor(hi, m));
-  }
+  auto join = [&](auto m) {
+    constexpr int M = decltype(m)::value;
+    lo = __builtin_elementwise_minimum(lo, xor_lane<M>(lo));
+    hi = __builtin_elementwise_maximum(hi, xor_lane<M>(hi));
+  };
+  join(std::integral_constant<int, 1>{});
+  join(std::integral_constant<int, 2>{});   // (a group is four lanes at least)
+  if (group_lanes >= 8) join(std::integral_constant<int, 4>{});
+  if constexpr (LPH >= 16)
+    if (group_lanes >= 16) join(std::integral_constant<int, 8>{});
+  if constexpr (LPH >= 32)
+    if (group_lanes >= 32) join(std::integral_constant<int, 16>{});
   const f16 s = (f16)((hi - lo) / 15.0f);
   const f16 c = (f16)(lo + 8.0f * (float)s);
   const float inv = 1.0f / (float)s;
-  const bool ok = __builtin_isfinite(inv) && __builtin_isfinite((float)c) &&
-                  __builtin_isfinite((float)s);
+  Codes r;
+  r.ok = __builtin_isfinite(inv) && __builtin_isfinite((float)c) && __builtin_isfinite((float)s);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float n = rintf((y[i] - (float)c) * inv);
-    code[i] = ok ? (uint32_t)((int)fminf(fmaxf(n, -8.0f), 7.0f) + 8) : 8u;
+    // held to [-8, 7], then rounded to even by the addition, whose result ends in the
+    // code's bits: 1.5 * 2^23 + 8 + n
+    const float n = __builtin_amdgcn_fmed3f((y[i] - (float)c) * inv, -8.0f, 7.0f);
+    r.code[i] = __builtin_bit_cast(uint32_t, n + 12582920.0f) & 15u;
   }
-  return (uint32_t)as_u16(s) | (uint32_t)as_u16(c) << 16;
+  r.group = (uint32_t)as_u16(s) | (uint32_t)as_u16(c) << 16;
+  return r;
 }
 
 __device__ __forceinline__ void unpack8(u32x4 v, uint16_t h[8]) {
@@ -132,49 +215,106 @@ __device__ __forceinline__ void unpack8(u32x4 v, uint16_t h[8]) {
   }
 }
 
-template <int LPH, bool BF16>
-__device__ __forceinline__ void qk_part(const RopeArgs& a, int block) {
-  constexpr int D = 8 * LPH;
-  const int heads = a.q_heads + a.kv_heads;
-  const int unit = block * (kThreads / LPH) + (int)threadIdx.x / LPH;
+template <bool BF16>
+__device__ __forceinline__ void widen(u32x4 v, float y[8]) {
+  uint16_t h[8];
+  unpack8(v, h);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = to_f32<BF16>(h[i]);
+}
+
+template <bool BF16>
+__device__ __forceinline__ u32x4 narrow(const float y[8]) {
+  u32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    r[i] = (uint32_t)from_f32<BF16>(y[2 * i]) | (uint32_t)from_f32<BF16>(y[2 * i + 1]) << 16;
+  return r;
+}
+
+// N heads a group of lanes, of one token's: x -> out.
+template <int LPH, bool BF16, int N>
+__device__ __forceinline__ void dense_part(const RopeArgs& a, int block, int parts,
+                                           const uint16_t* x, int64_t x_token, int64_t x_head,
+                                           const uint16_t* weight, uint16_t* out, int heads) {
+  static_assert(N == 1 || N == 4, "a quad's lanes share the square roots");
+  constexpr int D = 8 * LPH, kAtOnce = kThreads / LPH;
+  const int t = block / parts, part = block - t * parts;
   const int lane = threadIdx.x % LPH;
-  if (unit >= a.tokens * heads) return;
-  const int t = unit / heads, h = unit - t * heads;
-  const bool is_q = h < a.q_heads;
-  const int kh = h - a.q_heads;
-  const uint16_t* src = is_q ? a.q + t * a.q_token + h * a.q_head : a.k + t * a.k_token + kh * a.k_head;
-  uint16_t half8[8];
-  unpack8(load8(src + 8 * lane), half8);
-  float y[8];
+  const int h0 = part * kAtOnce * N + (int)threadIdx.x / LPH;   // and every kAtOnce-th after it
+  if (h0 >= heads) return;
+  const uint16_t* src = x + (int64_t)t * x_token + 8 * lane;
+  u32x4 raw[N];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = to_f32<BF16>(half8[i]);
-  const int pos = a.position[t];
-  norm_rotate<LPH, BF16>(y, a, is_q ? a.q_weight : a.k_weight, pos, lane);
-  if (is_q || !a.store) {
-    u32x4 r;
+  for (int j = 0; j < N; ++j)
+    raw[j] = load8(src + (int64_t)min(h0 + j * kAtOnce, heads - 1) * x_head);
+  const Turn turn = turn_of<LPH>(a, a.position[t], lane);
+  float w[8], r = 1.0f;
+  if (weight) {
+    widen<BF16>(load8(weight + 8 * lane), w);
+    float q = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      r[i] = (uint32_t)from_f32<BF16>(y[2 * i]) | (uint32_t)from_f32<BF16>(y[2 * i + 1]) << 16;
-    uint16_t* dst = is_q ? a.q_out + ((int64_t)t * a.q_heads + h) * D
-                         : a.k_out + ((int64_t)t * a.kv_heads + kh) * D;
-    *reinterpret_cast<u32x4*>(dst + 8 * lane) = r;
-    return;
+    for (int j = 0; j < N; ++j) {
+      float y[8];
+      widen<BF16>(raw[j], y);
+      const float qj = squares<LPH>(y);
+      q = N == 1 || (lane & 3) == j ? qj : q;
+    }
+    r = root<LPH>(q, a.eps);
   }
-  uint32_t code[8];
-  const uint32_t group = quantise(y, a.group_lanes, code);
-  const int row = a.rows ? a.rows[t] : t;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int h = h0 + j * kAtOnce;
+    if (h >= heads) return;
+    float y[8];
+    widen<BF16>(raw[j], y);
+    if (weight) {
+      const float rj = N == 1   ? r
+                       : j == 0 ? quad_lane<0>(r)
+                       : j == 1 ? quad_lane<1>(r)
+                       : j == 2 ? quad_lane<2>(r)
+                                : quad_lane<3>(r);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = (y[i] * rj) * w[i];
+    }
+    rotate<LPH>(y, a, turn);
+    *reinterpret_cast<u32x4*>(out + ((int64_t)t * heads + h) * D + 8 * lane) = narrow<BF16>(y);
+  }
+}
+
+// Stored keys: a group of lanes to a token's head.
+template <int LPH, bool BF16>
+__device__ __forceinline__ void key_part(const RopeArgs& a, int block) {
+  constexpr int D = 8 * LPH;
+  const int unit = block * (kThreads / LPH) + (int)threadIdx.x / LPH, lane = threadIdx.x % LPH;
+  if (unit >= a.tokens * a.kv_heads) return;
+  const int t = unit / a.kv_heads, h = unit - t * a.kv_heads;
+  const u32x4 raw = load8(a.k + (int64_t)t * a.k_token + (int64_t)h * a.k_head + 8 * lane);
+  const int pos = a.position[t], row = a.rows ? a.rows[t] : t;
+  const Turn turn = turn_of<LPH>(a, pos, lane);
   const int64_t page = pos < 0 ? -1 : kv4_page(a.table, a.table_rows, a.max_pages, a.pages, row,
                                                pos >> a.page_shift);
+  float y[8];
+  widen<BF16>(raw, y);
+  if (a.k_weight) {
+    float w[8];
+    widen<BF16>(load8(a.k_weight + 8 * lane), w);
+    const float r = root<LPH>(squares<LPH>(y), a.eps);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = (y[i] * r) * w[i];
+  }
+  rotate<LPH>(y, a, turn);
+  const Codes q = quantise<LPH>(y, a.group_lanes);
   if (page < 0) return;
   const int P = 1 << a.page_shift, tok = pos & (P - 1);
   const Kv4Layout f{P, D, a.NG};
-  int32_t* blk = a.pool + (page * a.kv_heads + kh) * f.words();
-  uint32_t w = 0;
+  int32_t* blk = a.pool + (page * a.kv_heads + h) * f.words();
+  uint32_t word = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w |= code[i] << kv4_shift(i);
-  blk[tok * (D / 8) + kv4_key_word(lane, D)] = (int32_t)w;
+  for (int i = 0; i < 8; ++i) word |= q.code[i] << kv4_shift(i);
+  blk[tok * (D / 8) + kv4_key_word(lane, D)] = (int32_t)(q.ok ? word : 0x88888888u);
   if (lane % a.group_lanes == 0)
-    blk[f.key_groups() + lane / a.group_lanes * P + tok] = (int32_t)group;
+    blk[f.key_groups() + lane / a.group_lanes * P + tok] = (int32_t)q.group;
 }
 
 constexpr int kChunk = 32;   // most tokens of a value chunk
@@ -182,17 +322,25 @@ constexpr int kChunk = 32;   // most tokens of a value chunk
 template <int LPH, bool BF16>
 __device__ __forceinline__ void value_part(const RopeArgs& a, int block) {
   constexpr int D = 8 * LPH;
-  __shared__ uint8_t codes[kChunk][D];
+  __shared__ __attribute__((aligned(8))) uint8_t codes[kChunk][D];
   __shared__ int64_t where[kChunk];      // block of the token's page and head, in words; -1: none
   __shared__ int place[kChunk];          // token within the page
-  __shared__ uint8_t member[kChunk][8];  // of the octet that a token leads: who holds which place
+  __shared__ __attribute__((aligned(8))) uint8_t member[kChunk][8];  // of the octet that a token leads: who holds which place
   __shared__ uint32_t leaders;
+  constexpr int kAtOnce = kThreads / LPH, kTurns = kChunk / kAtOnce;
   const int kh = block % a.kv_heads, t0 = block / a.kv_heads * a.chunk;
   const int n = min(a.chunk, a.tokens - t0);
   const int P = 1 << a.page_shift;
   const Kv4Layout f{P, D, a.NG};
-  const int lane = threadIdx.x % LPH;
-  if ((int)threadIdx.x < kChunk) {
+  const int lane = threadIdx.x % LPH, mine = threadIdx.x / LPH;
+  // the values first: they arrive while the pages are looked up
+  u32x4 raw[kTurns];
+#pragma unroll
+  for (int i = 0; i < kTurns; ++i) {
+    const int c = min(mine + i * kAtOnce, n - 1);
+    raw[i] = load8(a.v + (int64_t)(t0 + c) * a.v_token + (int64_t)kh * a.v_head + 8 * lane);
+  }
+  if (threadIdx.x < 64) {
     const int c = threadIdx.x;
     int64_t at = -1;
     int tok = 0;
@@ -203,41 +351,41 @@ __device__ __forceinline__ void value_part(const RopeArgs& a, int block) {
       tok = pos & (P - 1);
       if (page >= 0) at = (page * a.kv_heads + kh) * f.words();
     }
-    where[c] = at;
-    place[c] = tok;
-    for (int i = 0; i < 8; ++i) member[c][i] = 255;
+    if (c < kChunk) {
+      where[c] = at;
+      place[c] = tok;
+      *reinterpret_cast<u32x2*>(member[c]) = u32x2{~0u, ~0u};
+    }
+    // the first token of the chunk in an octet leads it: its words are at `octet`
+    const int64_t octet = at < 0 ? -1 : at + (tok >> 3);   // (P octets apart at least: unique)
+    uint64_t left = __ballot(at >= 0), all = 0;
+    while (left) {
+      const int lead = __builtin_ctzll(left);
+      const int64_t key =
+          (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)octet, lead) |
+                    (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(octet >> 32), lead)
+                        << 32);
+      const uint64_t same = __ballot(octet == key);
+      if (octet == key) member[lead][tok & 7] = (uint8_t)c;
+      all |= 1ull << lead;
+      left &= ~same;
+    }
+    if (c == 0) leaders = (uint32_t)all;
   }
   __syncthreads();
-  for (int c = threadIdx.x / LPH; c < n; c += kThreads / LPH) {
-    const uint16_t* src = a.v + (t0 + c) * a.v_token + kh * a.v_head;
-    uint16_t half8[8];
-    unpack8(load8(src + 8 * lane), half8);
+#pragma unroll
+  for (int i = 0; i < kTurns; ++i) {
+    const int c = mine + i * kAtOnce;
+    if (c >= n) break;
     float y[8];
+    widen<BF16>(raw[i], y);
+    const Codes q = quantise<LPH>(y, a.group_lanes);
+    u32x2 bytes = {0, 0};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = to_f32<BF16>(half8[i]);
-    uint32_t code[8];
-    const uint32_t group = quantise(y, a.group_lanes, code);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) codes[c][8 * lane + i] = (uint8_t)code[i];
+    for (int j = 0; j < 8; ++j) bytes[j / 4] |= q.code[j] << (8 * (j & 3));
+    *reinterpret_cast<u32x2*>(&codes[c][8 * lane]) = q.ok ? bytes : u32x2{0x08080808u, 0x08080808u};
     if (where[c] >= 0 && lane % a.group_lanes == 0)
-      a.pool[where[c] + f.value_groups() + lane / a.group_lanes * P + place[c]] = (int32_t)group;
-  }
-  if (threadIdx.x < 64) {
-    // the first token of the chunk in an octet leads it
-    const int c = threadIdx.x;
-    bool leads = false;
-    if (c < n && where[c] >= 0) {
-      int lead = c;
-      for (int o = 0; o < c; ++o)
-        if (where[o] == where[c] && place[o] >> 3 == place[c] >> 3) {
-          lead = o;
-          break;
-        }
-      member[lead][place[c] & 7] = (uint8_t)c;
-      leads = lead == c;
-    }
-    const uint64_t all = __ballot(leads);
-    if (c == 0) leaders = (uint32_t)all;
+      a.pool[where[c] + f.value_groups() + lane / a.group_lanes * P + place[c]] = (int32_t)q.group;
   }
   __syncthreads();
   // a wave takes a led octet's D words in rows of 64
@@ -268,14 +416,23 @@ __device__ __forceinline__ void value_part(const RopeArgs& a, int block) {
   }
 }
 
-template <int LPH, bool BF16>
+template <int LPH, bool BF16, int N>
 __global__ __launch_bounds__(kThreads) void kv4_rope_kernel(const RopeArgs a) {
-  if ((int)blockIdx.x < a.qk_blocks)
-    qk_part<LPH, BF16>(a, blockIdx.x);
-  else
-    value_part<LPH, BF16>(a, (int)blockIdx.x - a.qk_blocks);
+  // values first: their workgroups take longest
+  int block = blockIdx.x;
+  if (block < a.value_blocks) return value_part<LPH, BF16>(a, block);
+  block -= a.value_blocks;
+  if (block < a.k_blocks) {
+    if (a.store) return key_part<LPH, BF16>(a, block);
+    return dense_part<LPH, BF16, N>(a, block, a.k_parts, a.k, a.k_token, a.k_head, a.k_weight,
+                                    a.k_out, a.kv_heads);
+  }
+  dense_part<LPH, BF16, N>(a, block - a.k_blocks, a.q_parts, a.q, a.q_token, a.q_head, a.q_weight,
+                           a.q_out, a.q_heads);
 }
 
+// A group of lanes to a token's head; a workgroup has eight tokens that follow each
+// other and one, two or four heads, as eight tokens share every value word.
 struct ReadArgs {
   const int32_t *pool, *table, *rows, *position;
   uint16_t *k, *v;
@@ -285,10 +442,12 @@ struct ReadArgs {
 template <int LPH, bool BF16>
 __global__ __launch_bounds__(kThreads) void kv4_read_kernel(const ReadArgs a) {
   constexpr int D = 8 * LPH;
-  const int unit = (int)blockIdx.x * (kThreads / LPH) + (int)threadIdx.x / LPH;
-  const int lane = threadIdx.x % LPH;
-  if (unit >= a.tokens * a.heads) return;
-  const int t = unit / a.heads, h = unit - t * a.heads;
+  constexpr int kHeads = kThreads / LPH / 8;
+  const int lane = threadIdx.x % LPH, unit = threadIdx.x / LPH;
+  const int parts = (a.heads + kHeads - 1) / kHeads;
+  const int t = (int)blockIdx.x / parts * 8 + (unit & 7);
+  const int h = (int)blockIdx.x % parts * kHeads + (unit >> 3);
+  if (t >= a.tokens || h >= a.heads) return;
   const int pos = a.position[t], row = a.rows ? a.rows[t] : t;
   const int64_t page =
       pos < 0 ? -1 : kv4_page(a.table, a.table_rows, a.max_pages, a.pages, row, pos >> a.page_shift);
@@ -313,8 +472,9 @@ __global__ __launch_bounds__(kThreads) void kv4_read_kernel(const ReadArgs a) {
       rv[i / 2] |= (uint32_t)from_f32<BF16>(y) << (16 * (i & 1));
     }
   }
-  *reinterpret_cast<u32x4*>(a.k + (int64_t)unit * D + 8 * lane) = rk;
-  *reinterpret_cast<u32x4*>(a.v + (int64_t)unit * D + 8 * lane) = rv;
+  const int64_t at = ((int64_t)t * a.heads + h) * D + 8 * lane;
+  *reinterpret_cast<u32x4*>(a.k + at) = rk;
+  *reinterpret_cast<u32x4*>(a.v + at) = rv;
 }
 
 int log2_of(int x) { return __builtin_ctz((unsigned)x); }
@@ -333,7 +493,10 @@ hipError_t by_type(int D, bool bf16, const A& a, unsigned blocks, hipStream_t st
 template <int LPH, bool BF16>
 struct GoRope {
   static hipError_t go(const RopeArgs& a, unsigned blocks, hipStream_t st) {
-    kv4_rope_kernel<LPH, BF16><<<dim3(blocks), dim3(kThreads), 0, st>>>(a);
+    if (a.four)
+      kv4_rope_kernel<LPH, BF16, 4><<<dim3(blocks), dim3(kThreads), 0, st>>>(a);
+    else
+      kv4_rope_kernel<LPH, BF16, 1><<<dim3(blocks), dim3(kThreads), 0, st>>>(a);
     return hipGetLastError();
   }
 };
@@ -372,8 +535,17 @@ hipError_t launch_rope(const w4a16_rope& t, const w4a16_kv4* kv, const int32_t* 
   a.interleaved = (t.flags & W4A16_KV4_INTERLEAVED) != 0;
   const int D = t.head_dim;
   a.group_lanes = 1;
-  const int per_block = kThreads / (D / 8);
-  a.qk_blocks = (int)((t.tokens * (t.q_heads + t.kv_heads) + per_block - 1) / per_block);
+  // four heads a group of lanes where they are normed and that leaves every CU some
+  // workgroups (7192 tokens of 64 + 8 heads of 128: one head each 67 us, four 56; not
+  // normed, 4095 tokens of 64 heads of 64: one 13.6, four 17.2)
+  const int at_once = kThreads / (D / 8);
+  a.four = (t.q_weight || t.k_weight) &&
+           t.tokens * (t.q_heads + t.kv_heads) >= 4 * at_once * 1024;
+  const int each = at_once * (a.four ? 4 : 1);
+  a.q_parts = (t.q_heads + each - 1) / each;
+  a.q_blocks = (int)(t.tokens * a.q_parts);
+  a.k_parts = (t.kv_heads + each - 1) / each;
+  a.k_blocks = (int)(t.tokens * a.k_parts);
   if (kv) {
     a.store = true;
     a.v = static_cast<const uint16_t*>(t.v);
@@ -392,8 +564,9 @@ hipError_t launch_rope(const w4a16_rope& t, const w4a16_kv4* kv, const int32_t* 
     // single tokens of many sequences changes words one by one
     a.chunk = t.tokens * t.kv_heads < 32 * 512 ? 8 : kChunk;
     a.value_blocks = (int)((t.tokens + a.chunk - 1) / a.chunk * t.kv_heads);
+    a.k_blocks = (int)((t.tokens * t.kv_heads + at_once - 1) / at_once);
   }
-  const unsigned blocks = (unsigned)a.qk_blocks + (unsigned)a.value_blocks;
+  const unsigned blocks = (unsigned)a.q_blocks + (unsigned)a.k_blocks + (unsigned)a.value_blocks;
   return by_type<GoRope>(D, t.flags & W4A16_KV4_BF16, a, blocks, st);
 }
 
@@ -403,9 +576,9 @@ hipError_t launch_kv4_read(const w4a16_kv4& kv, const int32_t* positions, const 
   ReadArgs a{kv.pool, kv.table, rows, positions, static_cast<uint16_t*>(k),
              static_cast<uint16_t*>(v), (int)tokens, kv.heads, (int)kv.rows, (int)kv.max_pages,
              (int)kv.pages, log2_of(kv.page_size), kv.group_size / 8, D / kv.group_size};
-  const int per_block = kThreads / (D / 8);
-  return by_type<GoRead>(D, bf16, a, (unsigned)((tokens * kv.heads + per_block - 1) / per_block),
-                         st);
+  const int heads = kThreads / (D / 8) / 8;   // of a workgroup
+  return by_type<GoRead>(D, bf16, a,
+                         (unsigned)((tokens + 7) / 8 * ((kv.heads + heads - 1) / heads)), st);
 }
 
 }  // namespace w4a16

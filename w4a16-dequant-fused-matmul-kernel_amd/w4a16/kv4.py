@@ -52,6 +52,7 @@ class _Native:
     time a call."""
 
     def __getattr__(self, name):
+        _lib.load()   # an unusable library is an error, as everywhere
         try:
             mod = _lib.load_native(_ZKEY)
         except ImportError as e:

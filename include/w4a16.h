@@ -305,8 +305,8 @@ int w4a16_dequantize_f16(const int32_t* qweight, const void* scales, const void*
  *   the i-th of a word's eight codes lies in bits [4n, 4n+4), n = i/2 + 4*(i%2)
  *   keys: values 8o..8o+7 of a token in word (D/32) * (o % 4) + o/4 of its row
  *   values: value d of tokens 8u..8u+7 in word 64*(d/64) + 4*(d%16) + d/16 % 4
- * A group of numbers lo..hi is stored with scale = fp16((hi - lo) / 15), centre =
- * fp16(lo + 8 * scale), code = clamp(rint((x - centre) * (1 / scale)), -8, 7) + 8
+ * A group of numbers lo..hi is stored with scale = fp16((hi - lo) * (1/15)), centre
+ * = fp16(lo + 8 * scale), code = clamp(rint((x - centre) * (1 / scale)), -8, 7) + 8
  * (fp32, round to even); 8 where the scale is 0 or not finite.
  *
  * A page table is int32 [rows, max_pages]: one row per sequence, page ids in the

@@ -69,7 +69,7 @@ def quantise(x: torch.Tensor, G: int):
     """(codes, scales, centres) of fp32 x [..., D]; fp32 arithmetic as defined."""
     g = x.float().unflatten(-1, (-1, G))
     lo, hi = g.amin(-1, keepdim=True), g.amax(-1, keepdim=True)
-    s = ((hi - lo) / 15.0).half()
+    s = ((hi - lo) * (1.0 / 15.0)).half()
     c = (lo + 8.0 * s.float()).half()
     inv = 1.0 / s.float()
     ok = torch.isfinite(inv) & torch.isfinite(c.float()) & torch.isfinite(s.float())

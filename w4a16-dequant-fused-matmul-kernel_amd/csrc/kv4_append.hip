@@ -57,6 +57,13 @@ struct RopeArgs {
   bool interleaved, store, four;
 };
 
+// x as an fp32 number.  (A product and its rounding to fp16 would become one
+// instruction that rounds once.)
+__device__ __forceinline__ float rounded(float x) {
+  asm("" : "+v"(x));
+  return x;
+}
+
 // v of lane ^ M.  Within 16 lanes by DPP (quad permutations, a mirror of eight lanes
 // and a rotation by eight), which needs no LDS.
 template <int M>
@@ -191,8 +198,8 @@ __device__ __forceinline__ Codes quantise(const float y[8], int group_lanes) {
     if (group_lanes >= 16) join(std::integral_constant<int, 8>{});
   if constexpr (LPH >= 32)
     if (group_lanes >= 32) join(std::integral_constant<int, 16>{});
-  const f16 s = (f16)((hi - lo) / 15.0f);
-  const f16 c = (f16)(lo + 8.0f * (float)s);
+  const f16 s = (f16)rounded((hi - lo) * (1.0f / 15.0f));
+  const f16 c = (f16)rounded(lo + 8.0f * (float)s);
   const float inv = 1.0f / (float)s;
   Codes r;
   r.ok = __builtin_isfinite(inv) && __builtin_isfinite((float)c) && __builtin_isfinite((float)s);
@@ -228,7 +235,8 @@ __device__ __forceinline__ u32x4 narrow(const float y[8]) {
   u32x4 r;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    r[i] = (uint32_t)from_f32<BF16>(y[2 * i]) | (uint32_t)from_f32<BF16>(y[2 * i + 1]) << 16;
+    r[i] = (uint32_t)from_f32<BF16>(rounded(y[2 * i])) |
+           (uint32_t)from_f32<BF16>(rounded(y[2 * i + 1])) << 16;
   return r;
 }
 
@@ -468,8 +476,8 @@ __global__ __launch_bounds__(kThreads) void kv4_read_kernel(const ReadArgs a) {
     for (int i = 0; i < 8; ++i) {
       const float x = (float)((int)(kw >> kv4_shift(i) & 15) - 8) * ks + kc;
       const float y = (float)((int)(vw[kv4_value_word(8 * lane + i)] >> sh & 15) - 8) * vs + vc;
-      rk[i / 2] |= (uint32_t)from_f32<BF16>(x) << (16 * (i & 1));
-      rv[i / 2] |= (uint32_t)from_f32<BF16>(y) << (16 * (i & 1));
+      rk[i / 2] |= (uint32_t)from_f32<BF16>(rounded(x)) << (16 * (i & 1));
+      rv[i / 2] |= (uint32_t)from_f32<BF16>(rounded(y)) << (16 * (i & 1));
     }
   }
   const int64_t at = ((int64_t)t * a.heads + h) * D + 8 * lane;

@@ -25,6 +25,10 @@ int kv_check(const w4a16_kv4& kv) {
   if (kv.heads < 1 || kv.heads > 65535 || !size_ok(kv.pages) || !size_ok(kv.rows) ||
       !size_ok(kv.max_pages))
     return W4A16_ERR_BAD_SHAPE;
+  // a page's bytes are a 32-bit number in the kernels
+  if (kv.heads * (int64_t)kv.page_size * (kv.head_dim / 4 + 2 * (kv.head_dim / kv.group_size)) >
+      UINT32_MAX / 4)
+    return W4A16_ERR_BAD_SHAPE;
   if ((kv.pages && !kv.pool) || (kv.rows && kv.max_pages && !kv.table)) return W4A16_ERR_NULL_POINTER;
   return aligned(kv.pool, 16) && aligned(kv.table, 4) ? W4A16_OK : W4A16_ERR_BAD_PLAN;
 }

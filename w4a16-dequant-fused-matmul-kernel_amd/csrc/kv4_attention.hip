@@ -105,18 +105,22 @@ Kv4Plan kv4_attention_plan(const w4a16_kv4& kv, const w4a16_kv4_query& q) {
   const int64_t rows = q.max_q * per_kv;
   p.rows_form = rows > 32;
   p.cols = rows > 16 && kv.head_dim < 256 ? 2 : 1;
-  const int64_t tile_rows = p.rows_form ? 64 * p.cols : 16 * p.cols;
+  const int64_t tile_rows = 16 * p.cols;
   p.tiles = (int)((rows + tile_rows - 1) / tile_rows);
   int64_t span = q.max_context;
   if (q.window > 0) span = span < q.window + q.max_q ? span : q.window + q.max_q;
   const int64_t blocks = (span + 31) / 32 + 1;
-  // enough workgroups for every CU to hold a few, and for rows of unlike lengths to
-  // even out; a split has at least four blocks a wave
-  const int64_t units = q.batch * kv.heads * p.tiles, least = p.rows_form ? 8 : 16;
-  #ifndef KV4_TARGET
-#define KV4_TARGET 1024
-#endif
-  int64_t want = ((p.rows_form ? 512 : KV4_TARGET) + units - 1) / units;
+  // Four waves to some rows: about 1024 workgroups hold the chip's loads under way and
+  // let rows of unlike lengths even out (46 sequences to 8192 tokens: 768 workgroups
+  // 74 us, 1024 64, 2048 65); a split has a block a wave at least, and up to 16
+  // blocks are not split, as joining takes 3 us and a block about 1.
+  // A wave to some rows: split only where that leaves half the chip's waves unused
+  // (512 queries on 4000 tokens, 512 waves: two splits 95 us, four 82; 1266 on 2472,
+  // 1272 waves: one 122, two 137).
+  const int64_t units = q.batch * kv.heads * p.tiles, least = p.rows_form ? 8 : 4;
+  int64_t want = p.rows_form ? (units >= 1024 ? 1 : (2048 + units - 1) / units)
+                 : blocks <= 16 ? 1
+                                : (1024 + units - 1) / units;
   const int64_t most = (blocks + least - 1) / least;
   if (want > most) want = most;
   if (want < 1) want = 1;
@@ -167,7 +171,7 @@ hipError_t launch_kv4_attention(const Kv4Attn& c, hipStream_t st) {
                        : c.cols == 2 ? launch_attention_tokens2(a, D, NG, st)
                                      : launch_attention_tokens1(a, D, NG, st);
   if (e != hipSuccess || c.splits == 1) return e;
-  const int tile_rows = c.rows_form ? 64 * c.cols : 16 * c.cols;
+  const int tile_rows = 16 * c.cols;
   const int max_rows = (int)q.max_q * a.per_kv;
   switch (D) {
     case 64: launch_join<64>(a, tile_rows, max_rows, st); break;

@@ -17,17 +17,18 @@
 // packed subtraction makes it code - 8, exactly: nine instructions a word.
 //
 // The weights p s of the values are rounded to fp16 (to nearest), the only rounding
-// below 32 bits; it acts on code - 8, the centres' sum stays in fp32.  They are
-// scaled by 2^(7 - E), E the exponent of the largest scale met so far: fp16 then
-// holds every weight down to 2^-29 of the largest to its full precision.  Scores,
-// maxima, denominators and all sums are fp32.
+// below 32 bits; it acts on code - 8, the centres' sum stays in fp32.  The reference
+// that the scores' exponents are taken against is the running maximum plus E - 7, E
+// the exponent of the largest value scale met so far: weights end below 2^15, and
+// fp16 holds each down to 2^-29 of the largest to its full precision.  Scores,
+// references, denominators and all sums are fp32.
 //
 // A wave has 16 * C query rows and takes 32 tokens at a time: tokens are the rows
 // of the first product (two tiles of 16), so a lane holds the scores of one query
 // row and eight consecutive tokens, exactly the second product's operand.  The
-// running maximum moves only when a score exceeds it by 2^8 (or a value scale the
-// range above): then the sums are rescaled, else they are left alone, and the
-// branch is the wave's.
+// reference moves only when a score exceeds the maximum in it by 2^8, or a value scale
+// 2^E: then the sums are rescaled, else they are left alone, and the branch is the
+// wave's.
 //
 // Rows whose tokens are all hidden keep a denominator of 0 and become zeros.
 // Hidden tokens, and what lies behind the last one in a page, may hold anything:
@@ -39,8 +40,8 @@
 
 namespace w4a16 {
 
-constexpr int kAttnThreads = 256;
-constexpr float kNoScore = -1e30f;   // running maximum (in powers of two) before any score
+constexpr int kAttnThreads = 256;   // of a workgroup whose waves share their rows
+constexpr float kNoScore = -1e30f;   // reference (a power of two) before any score
 
 struct AttnArgs {
   const uint16_t* q;
@@ -83,6 +84,7 @@ __device__ __forceinline__ AttnSpan attn_span(const AttnArgs& a, int b, int r0, 
   return s;
 }
 
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) uint32_t lds_dword;
 typedef __attribute__((address_space(1))) uint32_t glb_dword;
 typedef __attribute__((address_space(4))) int32_t const_dword;   // read by scalar loads
@@ -223,8 +225,9 @@ struct AttnWave {
   float fac[C];                // score in powers of two = x * fac
   int see_lo[C], see_hi[C];    // tokens that the lane's row sees
   f32x4 acc[C][kTiles];
-  float m[C], l[C], csum[C][NG];
+  float ref[C], l[C], csum[C][NG];   // the reference; sums of p and p c
   int E;
+  uint16_t limit;   // 2^E as fp16: scales from this on move the reference
   MagicRegs mg;
 
   __device__ __forceinline__ void start() {
@@ -234,10 +237,11 @@ struct AttnWave {
       for (int i = 0; i < kTiles; ++i) acc[c][i] = f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int n = 0; n < NG; ++n) csum[c][n] = 0.0f;
-      m[c] = kNoScore;
+      ref[c] = kNoScore;
       l[c] = 0.0f;
     }
     E = -24;
+    limit = 1;
     mg = make_magic();
   }
 
@@ -305,113 +309,127 @@ struct AttnWave {
   // 32 tokens from t on.  `mask`: some of them are hidden from some row.
   __device__ __forceinline__ void step(const uint32_t* lds, int t, int lane, bool mask) {
     typedef Stage<D, NG> S;
-    const int g = lane >> 4, mine = t + 8 * g;
+    const int mine = t + 8 * (lane >> 4);   // the first of the lane's tokens
     float sc[C][8];
-    uint32_t kg[NG][8], vg[NG][8];
+    uint32_t kg[NG][8], vg[NG][8], kw[2][kSteps];
+    // (reads from LDS stand a phase ahead of their use, and both tiles' products
+    // before the first score: a wave would wait for each otherwise)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) S::keys(lds, j, lane, kw[j]);
 #pragma unroll
     for (int n = 0; n < NG; ++n) S::key_groups(lds, n, lane, kg[n]);
+    __builtin_amdgcn_sched_barrier(0);
+    f32x4 s[2][C][NG];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      uint32_t kw[kSteps];
-      S::keys(lds, j, lane, kw);
-      f32x4 s[C][NG];
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
           const float z = -8.0f * Q[c][n];
-          s[c][n] = f32x4{z, z, z, z};
+          s[j][c][n] = f32x4{z, z, z, z};
         }
 #pragma unroll
       for (int k = 0; k < kSteps; ++k) {
-        const f16x8 w = code_halves(kw[k]);
+        const f16x8 w = code_halves(kw[j][k]);
 #pragma unroll
         for (int c = 0; c < C; ++c)
-          s[c][k / (kSteps / NG)] =
-              __builtin_amdgcn_mfma_f32_16x16x32_f16(w, q[c][k], s[c][k / (kSteps / NG)], 0, 0, 0);
+          s[j][c][k / (kSteps / NG)] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+              w, q[c][k], s[j][c][k / (kSteps / NG)], 0, 0, 0);
       }
+    }
+#pragma unroll
+    for (int n = 0; n < NG; ++n) S::value_groups(lds, n, lane, vg[n]);
+    // (a term of all scores before the next: a mixed fma cannot be followed by one
+    // that takes its result)
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float v = 0.0f;
+        for (int i = 0; i < 8; ++i) {
+          sc[c][i] = fmaf(hi_f32(kg[n][i]), Q[c][n], n ? sc[c][i] : 0.0f);
+          asm volatile("" : "+v"(sc[c][i]));
+        }
 #pragma unroll
-          for (int n = 0; n < NG; ++n) {
-            v = fmaf(hi_f32(kg[n][4 * j + r]), Q[c][n], v);
-            v = fmaf(lo_f32(kg[n][4 * j + r]), s[c][n][r], v);
-          }
-          sc[c][4 * j + r] = v;
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          sc[c][i] = fmaf(lo_f32(kg[n][i]), s[i / 4][c][n][i % 4], sc[c][i]);
+          asm volatile("" : "+v"(sc[c][i]));
         }
     }
-    auto hidden = [&](int c, int i) { return mine + i < see_lo[c] || mine + i >= see_hi[c]; };
+    auto hidden = [&](int c, int i) { return see_lo[c] - mine > i || see_hi[c] - mine <= i; };
     if (mask) {
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int i = 0; i < 8; ++i) sc[c][i] = hidden(c, i) ? -__builtin_inff() : sc[c][i];
     }
-#pragma unroll
-    for (int n = 0; n < NG; ++n) S::value_groups(lds, n, lane, vg[n]);
     if (mask) {   // what no row sees may hold anything
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (mine + i < any_lo || mine + i >= any_hi) {
+        if (any_lo - mine > i || any_hi - mine <= i) {
 #pragma unroll
           for (int n = 0; n < NG; ++n) vg[n][i] = 0;
         }
     }
-    float big = 0.0f, sv[NG][8];
-    const float f = ldexpf(1.0f, 7 - E);
+    uint32_t vw[D / 16];
+#pragma unroll
+    for (int h = 0; h < D / 64; ++h) S::values(lds, h, lane, vw + 4 * h);
+    // the largest scale in the low half (none is negative; a NaN counts as large)
+    u16x2 most = {0, 0};
 #pragma unroll
     for (int n = 0; n < NG; ++n)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        sv[n][i] = fmaf(lo_f32(vg[n][i]), f, 0.0f);
-        big = fmaxf(big, sv[n][i]);
-      }
+      for (int i = 0; i < 8; ++i)
+        most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, vg[n][i]));
     float top[C];
-    bool move = !(big <= 128.0f);
+    const float room = 15.0f - (float)E;   // p <= 2^room keeps the weights below 2^15
+    bool move = most.x >= limit;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       top[c] = fmaxf(fmaxf(fmaxf(sc[c][0], sc[c][1]), fmaxf(sc[c][2], sc[c][3])),
                      fmaxf(fmaxf(sc[c][4], sc[c][5]), fmaxf(sc[c][6], sc[c][7])));
-      move |= top[c] * fac[c] > m[c] + 8.0f;
+      move |= top[c] * fac[c] > ref[c] + room;
     }
     if (__ballot(move)) {
-      // (scales times 2^(7 - E); an infinite one spoils the rows that see it, and
-      // must not move the others' range)
-      float fine = 0.0f;
+      // (an infinite scale spoils the rows that see it, and must not move the others')
+      float s = 0.0f;
 #pragma unroll
       for (int n = 0; n < NG; ++n)
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          fine = fmaxf(fine, sv[n][i] < __builtin_inff() ? sv[n][i] : 0.0f);
-      const float most = ldexpf(max_rows(fine), E - 7);
-      const int E1 = max(E, __builtin_amdgcn_readfirstlane(most > 0.0f ? __builtin_amdgcn_frexp_expf(most) : -24));
-      const float down = ldexpf(1.0f, E - E1);
+        for (int i = 0; i < 8; ++i) {
+          const float x = lo_f32(vg[n][i]);
+          s = fmaxf(s, x < __builtin_inff() ? x : 0.0f);
+        }
+      s = max_rows(s);
+      const int E1 = max(E, __builtin_amdgcn_readfirstlane(
+                                s > 0.0f ? __builtin_amdgcn_frexp_expf(s) : -24));
+      const float was = (float)(E - 7), now = (float)(E1 - 7);
+      const bool wider = E1 != E;
       E = E1;
+      limit = __builtin_bit_cast(uint16_t, (f16)ldexpf(1.0f, E));   // (2^16: infinity)
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        const float m1 = fmaxf(m[c], max_rows(top[c]) * fac[c]);
-        const float alpha = exp2f(m[c] - m1), all = alpha * down;
-        m[c] = m1;
+        // (rows that need no other reference keep theirs)
+        const float t = max_rows(top[c]) * fac[c];
+        const float to = wider || t > ref[c] + room ? fmaxf(ref[c] - was, t) + now : ref[c];
+        const float alpha = __builtin_amdgcn_exp2f(ref[c] - to);
+        ref[c] = to;
         l[c] *= alpha;
 #pragma unroll
         for (int n = 0; n < NG; ++n) csum[c][n] *= alpha;
 #pragma unroll
-        for (int i = 0; i < kTiles; ++i) acc[c][i] *= all;
+        for (int i = 0; i < kTiles; ++i) acc[c][i] *= alpha;
       }
-#pragma unroll
-      for (int n = 0; n < NG; ++n)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sv[n][i] *= down;
     }
     f16x8 w[C][NG];
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(sc[c][i], fac[c], -m[c]));
+        const float p = __builtin_amdgcn_exp2f(fmaf(sc[c][i], fac[c], -ref[c]));
         l[c] += p;
         sc[c][i] = p;
       }
@@ -423,7 +441,7 @@ struct AttnWave {
           const bool gone = hidden(c, i);
 #pragma unroll
           for (int n = 0; n < NG; ++n) {
-            w[c][n][i] = (f16)(gone ? 0.0f : sc[c][i] * sv[n][i]);
+            w[c][n][i] = (f16)(gone ? 0.0f : sc[c][i] * lo_f32(vg[n][i]));
             csum[c][n] = fmaf(sc[c][i], gone ? 0.0f : hi_f32(vg[n][i]), csum[c][n]);
           }
         }
@@ -434,23 +452,17 @@ struct AttnWave {
         for (int i = 0; i < 8; ++i)
 #pragma unroll
           for (int n = 0; n < NG; ++n) {
-            w[c][n][i] = (f16)(sc[c][i] * sv[n][i]);
+            w[c][n][i] = (f16)fmaf(sc[c][i], lo_f32(vg[n][i]), 0.0f);
             csum[c][n] = fmaf(sc[c][i], hi_f32(vg[n][i]), csum[c][n]);
           }
     }
 #pragma unroll
-    for (int h = 0; h < D / 64; ++h) {
-      uint32_t vw[4];
-      S::values(lds, h, lane, vw);
+    for (int i = 0; i < kTiles; ++i) {
+      const f16x8 v = value_halves(vw[i], mg);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const f16x8 v = value_halves(vw[j], mg);
-        const int i = 4 * h + j;
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-          acc[c][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[c][i / (kTiles / NG)], acc[c][i],
-                                                             0, 0, 0);
-      }
+      for (int c = 0; c < C; ++c)
+        acc[c][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[c][i / (kTiles / NG)], acc[c][i],
+                                                           0, 0, 0);
     }
   }
 
@@ -477,7 +489,7 @@ struct AttnWave {
       for (int i = 0; i < kTiles; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          acc[c][i][j] = ldexpf(acc[c][i][j], E - 7) + csum[c][i / (kTiles / NG)];
+          acc[c][i][j] += csum[c][i / (kTiles / NG)];
     }
   }
 };
@@ -516,21 +528,11 @@ struct PageOf {
   }
 };
 
-// Buffers of 32 tokens a wave (or, rows form, of 64 a workgroup) that are filled in
-// turn: one on its way while one is worked on.  A third one costs more waves on a CU
-// than it brings (220 MB of cache, 46 sequences: 81 us with three, 67 with two).
-#ifndef KV4_S
-#define KV4_S 2
-#endif
-constexpr int kStages = KV4_S;
+// Buffers of 32 tokens a wave that are filled in turn: one on its way while one is
+// worked on.  A third one costs more waves on a CU than it brings (220 MB of cache,
+// 46 sequences: 81 us with three, 67 with two).
+constexpr int kStages = 2;
 
-// kRows false: the four waves share 16 * C rows and take blocks of 32 tokens in turn,
-// each through buffers of its own; true: each has 16 * C rows of its own, and all
-// go through the workgroup's blocks together, 64 tokens at a time.  Grid: kv head
-// fastest (an XCD then keeps to few heads and finds their codes in its L2), then
-// sequence, split, and the row tiles from the last, which sees the most tokens, to
-// the first.  (Splits before sequences put the empty splits of short sequences on
-// the same CUs: 46 sequences of 1 to 8192 tokens in 4 splits 85 us, in 3 65.)
 // Waves per SIMD that the registers allow without spilling.  Nothing may spill: the
 // loop's counted waits take every load for one of its own.
 template <int D, int NG, int C>
@@ -538,42 +540,49 @@ constexpr int kWaves = C == 1 && D + 32 * NG <= 160   ? 4
                        : C == 1 && D + 32 * NG <= 192 ? 3
                        : C * (D + 32 * (NG - 1)) <= 320 ? 2 : 1;
 
+// A workgroup is four waves that share 16 * C rows and take blocks of 32 tokens in
+// turn, or (kRows) one wave that takes all of them.  (Four waves with rows of their
+// own and the same buffers wait for each other and leave larger pieces: prompts of
+// 2048 and 1266 tokens 361 us, single waves 334.)  Grid: kv head fastest (an XCD
+// then keeps to few heads and finds their codes in its L2), then sequence, split,
+// and the row tiles from the last, which sees the most tokens, to the first.  (Splits
+// before sequences put the empty splits of short sequences on the same CUs: 46
+// sequences of 1 to 8192 tokens in 4 splits 85 us, in 3 65.)
 template <int D, int NG, int C, bool kRows>
-__global__ __launch_bounds__(kAttnThreads, (kWaves<D, NG, C>)) void kv4_attention_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(kRows ? 64 : kAttnThreads, (kWaves<D, NG, C>)) void
+kv4_attention_kernel(const AttnArgs a) {
   typedef Stage<D, NG> S;
-  constexpr int kTiles = D / 16, kS = kStages;
-  constexpr int kRing = kRows ? kS * 2 * S::kWords : 4 * kS * S::kWords;
+  constexpr int kTiles = D / 16, kS = kStages, kShare = kRows ? 1 : 4;
+  constexpr int kRing = kShare * kS * S::kWords;
   // the four waves' results (rows 4 floats apart beyond D: the four groups of lanes
   // use different banks), then their maxima and denominators
   constexpr int kSumRow = D + 4, kSum = kRows ? 0 : 4 * 16 * kSumRow + 4 * 16 * 2;
   __shared__ __attribute__((aligned(16))) uint32_t lds[kRing > kSum ? kRing : kSum];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int wave = kRows ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint32_t id = blockIdx.x;
   const int h = id % a.heads;
   id /= a.heads;
   const int b = id % a.batch;
   id /= a.batch;
   const int split = id % a.splits, tile = a.tiles - 1 - (int)(id / a.splits);
-  const int rows = kRows ? 64 * C : 16 * C;
-  const int r0 = tile * rows;
-  const AttnSpan s = attn_span(a, b, r0, rows);
+  const int r0 = tile * 16 * C;   // the first row
+  const AttnSpan s = attn_span(a, b, r0, 16 * C);
   const int R = s.nq * a.per_kv;
   if (r0 >= R) return;
   if (a.splits > 1 && split >= s.active) return;
-  const int w0 = kRows ? r0 + wave * 16 * C : r0;   // the wave's first row
 
   // queries first, then the first blocks; the queries are worked on meanwhile
   AttnWave<D, NG, C> w;
 #pragma unroll
-  for (int c = 0; c < C; ++c) w.load_row(a, s, h, w0 + 16 * c + (lane & 15), c, lane);
+  for (int c = 0; c < C; ++c) w.load_row(a, s, h, r0 + 16 * c + (lane & 15), c, lane);
   // (rows past the last query see nothing, and need no mask to be ignored)
-  const int p0 = s.n - s.nq + w0 / a.per_kv;   // positions of the first and last query
-  const int p1 = s.n - s.nq + min((w0 + 16 * C - 1) / a.per_kv, s.nq - 1);
+  const int p0 = s.n - s.nq + r0 / a.per_kv;   // positions of the first and last query
+  const int p1 = s.n - s.nq + min((r0 + 16 * C - 1) / a.per_kv, s.nq - 1);
   w.all_hi = a.causal ? min(max(p0 + 1, 0), s.n) : s.n;
   w.any_hi = a.causal ? min(max(p1 + 1, 0), s.n) : s.n;
   w.any_lo = a.window > 0 ? min(max(0, p0 - a.window + 1), w.any_hi) : 0;
   w.all_lo = a.window > 0 ? max(0, p1 - a.window + 1) : 0;
-  if (w0 >= R) w.any_hi = 0;
   w.start();
   {
     // the split's blocks
@@ -590,77 +599,35 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<D, NG, C>)) void kv4_attentio
     auto block = [&](int pg) {   // (a missing page's loads go to page 0, unused)
       return head + (uint64_t)(uint32_t)max(pg, 0) * page_bytes;
     };
-    if constexpr (kRows) {
-      // wave w makes loads w, w + 4, ... of a pair of blocks; the last again where
-      // they do not come out even, so that all waves count the same
-      constexpr int kPair = 2 * S::kLoads, kMine = (kPair + 3) / 4;
-      uint32_t there = 0;   // two bits a buffer
-      auto fill = [&](int slot, int kb) {
-        const int k1 = min(kb + 1, end - 1);
-        const int pg0 = page(kb), pg1 = page(k1);
-        there = (there & ~(3u << (2 * slot))) |
-                ((pg0 >= 0 ? 1u : 0u) | (pg1 >= 0 && kb + 1 < end ? 2u : 0u)) << (2 * slot);
-        const char *b0 = block(pg0), *b1 = block(pg1);
-        uint32_t* to = lds + slot * 2 * S::kWords;
+    uint32_t* mine = lds + wave * kS * S::kWords;
+    uint32_t there = 0;
+    int next = first + wave, pg = next < end ? page(next) : -1;   // the next to fill
+    auto fill = [&](int slot) {
+      there = (there & ~(1u << slot)) | (pg >= 0 ? 1u : 0u) << slot;
+      const char* from = block(pg);
 #pragma unroll
-        for (int i = 0; i < kPair; ++i)
-          if (i % 4 == wave || (i == kPair - 1 && kPair % 4 && wave >= kPair % 4))
-            stage.load(i % S::kLoads, i < S::kLoads ? b0 : b1, P,
-                       ((i < S::kLoads ? kb : k1) << 5) & (P - 1),
-                       to + (i < S::kLoads ? 0 : S::kWords));
-      };
+      for (int i = 0; i < S::kLoads; ++i)
+        stage.load(i, from, P, (next << 5) & (P - 1), mine + slot * S::kWords);
+      next += kShare;
+      pg = page(min(next, end - 1));   // (asked for a block ahead of its use)
+    };
 #pragma unroll
-      for (int i = 0; i < kS - 1; ++i)
-        if (first + 2 * i < end) fill(i, first + 2 * i);
-      w.convert(a);
-      int slot = 0;
-      for (int kb = first; kb < end; kb += 2) {
-        // this pair is there, by every wave's loads, and the last one read by all
-        if (kS == 3 && kb + 2 < end)
-          wait_loads<kMine>();
-        else
-          wait_loads<0>();
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        const int last = slot == 0 ? kS - 1 : slot - 1;
-        if (kb + 2 * (kS - 1) < end) fill(last, kb + 2 * (kS - 1));
-        const uint32_t* x = lds + slot * 2 * S::kWords;
-        w.block(x, kb, there >> (2 * slot) & 1, lane);
-        w.block(x + S::kWords, kb + 1, there >> (2 * slot) & 2, lane);
-        slot = slot + 1 == kS ? 0 : slot + 1;
+    for (int i = 0; i < kS - 1; ++i)
+      if (next < end) fill(i);
+    w.convert(a);
+    int slot = 0;
+    for (int kb = first + wave; kb < end; kb += kShare) {
+      const int last = slot == 0 ? kS - 1 : slot - 1;
+      if (next < end) {
+        // (what was read of this buffer has been used: its last values fed products)
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        fill(last);
+        wait_loads<(kS - 1) * S::kLoads>();
+      } else {
+        wait_loads<0>();
       }
-    } else {
-      uint32_t* mine = lds + wave * kS * S::kWords;
-      uint32_t there = 0;
-      int next = first + wave, pg = page(min(next, max(end - 1, 0)));   // the next to fill
-      auto fill = [&](int slot) {
-        there = (there & ~(1u << slot)) | (pg >= 0 ? 1u : 0u) << slot;
-        const char* from = block(pg);
-#pragma unroll
-        for (int i = 0; i < S::kLoads; ++i)
-          stage.load(i, from, P, (next << 5) & (P - 1), mine + slot * S::kWords);
-        next += 4;
-        pg = page(min(next, end - 1));   // (asked for a block ahead of its use)
-      };
-#pragma unroll
-      for (int i = 0; i < kS - 1; ++i)
-        if (next < end) fill(i);
-      w.convert(a);
-      int slot = 0;
-      for (int kb = first + wave; kb < end; kb += 4) {
-        const int last = slot == 0 ? kS - 1 : slot - 1;
-        if (next < end) {
-          // (what was read of this buffer has been used: its last values fed products)
-          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-          fill(last);
-          wait_loads<(kS - 1) * S::kLoads>();
-        } else if (kS == 3 && kb + 4 < end) {
-          wait_loads<S::kLoads>();
-        } else {
-          wait_loads<0>();
-        }
-        w.block(mine + slot * S::kWords, kb, there >> slot & 1, lane);
-        slot = slot + 1 == kS ? 0 : slot + 1;
-      }
+      w.block(mine + slot * S::kWords, kb, there >> slot & 1, lane);
+      slot = slot + 1 == kS ? 0 : slot + 1;
     }
   }
   w.finish();
@@ -669,7 +636,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<D, NG, C>)) void kv4_attentio
   if constexpr (kRows) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const int r = w0 + 16 * c + col;
+      const int r = r0 + 16 * c + col;
       if (r >= R) continue;
       const int i = r / a.per_kv;
       const int64_t qrow = (int64_t)(s.q0 + i) * a.q_heads + h * a.per_kv + (r - i * a.per_kv);
@@ -679,7 +646,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<D, NG, C>)) void kv4_attentio
         for (int t = 0; t < kTiles; ++t) *reinterpret_cast<f32x4*>(dst + 16 * t + 4 * g) = w.acc[c][t];
         if (g == 0) {
           float* ml = part_ml(a, split, qrow, D);
-          ml[0] = w.m[c];
+          ml[0] = w.ref[c];
           ml[1] = w.l[c];
         }
       } else {
@@ -692,7 +659,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<D, NG, C>)) void kv4_attentio
           for (int j = 0; j < 4; ++j) v[j] = any ? w.acc[c][t][j] * inv : 0.0f;
           store4(a.out + qrow * D + 16 * t + 4 * g, v, a.bf16);
         }
-        if (a.lse && g == 0) a.lse[qrow] = lse_of(w.m[c], w.l[c]);
+        if (a.lse && g == 0) a.lse[qrow] = lse_of(w.ref[c], w.l[c]);
       }
     }
   } else {
@@ -703,12 +670,12 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<D, NG, C>)) void kv4_attentio
     for (int c = 0; c < C; ++c) {
       if (c) __syncthreads();
       if (g == 0) {
-        ml[wave][col][0] = w.m[c];
+        ml[wave][col][0] = w.ref[c];
         ml[wave][col][1] = w.l[c];
       }
       __syncthreads();
       const float m1 = fmaxf(fmaxf(ml[0][col][0], ml[1][col][0]), fmaxf(ml[2][col][0], ml[3][col][0]));
-      const float mine = exp2f(w.m[c] - m1);
+      const float mine = exp2f(w.ref[c] - m1);
 #pragma unroll
       for (int t = 0; t < kTiles; ++t)
         *reinterpret_cast<f32x4*>(&sum[wave][col][16 * t + 4 * g]) = w.acc[c][t] * mine;
@@ -754,7 +721,8 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<D, NG, C>)) void kv4_attentio
 // One form of the kernel for every head size and group count.
 template <int C, bool kRows>
 hipError_t launch_attention_form(const AttnArgs& a, int D, int NG, hipStream_t st) {
-  const dim3 grid((unsigned)a.heads * a.splits * a.batch * a.tiles), block(kAttnThreads);
+  const dim3 grid((unsigned)a.heads * a.splits * a.batch * a.tiles);
+  const dim3 block(kRows ? 64 : kAttnThreads);
   switch (D == 256 ? 0 : D * 8 + NG) {
     case 64 * 8 + 1: kv4_attention_kernel<64, 1, C, kRows><<<grid, block, 0, st>>>(a); break;
     case 64 * 8 + 2: kv4_attention_kernel<64, 2, C, kRows><<<grid, block, 0, st>>>(a); break;

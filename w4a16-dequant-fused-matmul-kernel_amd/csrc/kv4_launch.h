@@ -16,10 +16,9 @@ hipError_t launch_rope(const w4a16_rope& t, const w4a16_kv4* kv, const int32_t* 
 hipError_t launch_kv4_read(const w4a16_kv4& kv, const int32_t* positions, const int32_t* rows,
                            int64_t tokens, void* k, void* v, bool bf16, hipStream_t st);
 
-// One attention call, planned (kv4_attention_plan).  A workgroup has four waves.
-//   rows_form: each wave has 16 * cols query rows of its own and all keys of the
-//              workgroup's range; else all waves have the same 16 * cols rows and
-//              take 32-token blocks in turn.
+// One attention call, planned (kv4_attention_plan).  A workgroup has 16 * cols query
+// rows; four waves that take 32-token blocks in turn, or (rows_form) one wave that
+// takes all of its range.
 // `chunk` blocks of 32 tokens to a split, the last split to the end; splits > 1
 // leave fp32 partials (unnormalised sums, then maximum and denominator) in `part`.
 struct Kv4Attn {

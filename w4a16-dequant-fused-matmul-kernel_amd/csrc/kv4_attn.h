@@ -563,9 +563,14 @@ kv4_attention_kernel(const AttnArgs a) {
   uint32_t id = blockIdx.x;
   const int h = id % a.heads;
   id /= a.heads;
-  const int b = id % a.batch;
+  const uint32_t b0 = id % a.batch;
   id /= a.batch;
   const int split = id % a.splits, tile = a.tiles - 1 - (int)(id / a.splits);
+  // An XCD's workgroups go to its four groups of CUs in turn: an even number of
+  // sequences is turned on from tile to tile, so that a long one's do not all fall on
+  // the same group (two prompts, 2048 and 1266 tokens: 349 us without, 287 with)
+  const uint32_t turn = a.batch & 1 ? 0 : a.batch & 2 ? id >> 1 : id;
+  const int b = (b0 + turn) % a.batch;
   const int r0 = tile * 16 * C;   // the first row
   const AttnSpan s = attn_span(a, b, r0, 16 * C);
   const int R = s.nq * a.per_kv;

@@ -789,3 +789,140 @@ def test_layer_prefill_decode_fork_compact():
     used = cache.table[cache.table >= 0]
     assert live == len(used.unique()) and int(used.max()) == live - 1
     step([3, 2, 4, 0], [2, 1, 1, 40], 4, lens)
+
+
+def test_decode_step_in_a_graph():
+    """Extending, storing and attending captured once and replayed, with eager work in
+    between, fill a cache as eager steps do; pages are taken as they are needed."""
+    from w4a16 import KV4Cache
+
+    H, Hq, D, P, B = 2, 4, 64, 32, 3
+    cos, sin = (x.to(DEV) for x in _rotation(256, D))
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)   # noqa: E731
+    rows = i32([4, 0, 2])
+    ones = i32([1] * B)
+    qkv = torch.empty(B, Hq + 2 * H, D, dtype=torch.float16, device=DEV)
+    inputs = [torch.randn(qkv.shape, generator=_gen(i)).half().to(DEV) for i in range(40)]
+
+    def make():
+        c = KV4Cache(2, 12, H, D, sequences=5, max_pages=4, page_size=P, group_size=32, device=DEV)
+        return c, torch.zeros(B, dtype=torch.int32, device=DEV)
+
+    def step(c, pos):
+        c.extend(rows, ones)
+        y = None
+        for layer in range(2):
+            q = c.append(layer, qkv[:, :Hq], qkv[:, Hq:Hq + H], qkv[:, Hq + H:], cos, sin, pos, rows)
+            y = c.attend(layer, q, seqs=rows, max_context=128)
+        pos += 1
+        return y
+
+    eager, pos = make()
+    want = []
+    for x in inputs:
+        qkv.copy_(x)
+        want.append(step(eager, pos).clone())
+    cache, pos = make()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = step(cache, pos)
+    for i, x in enumerate(inputs):
+        qkv.copy_(x)
+        g.replay()
+        assert torch.equal(y, want[i]), i
+        if i % 7 == 0:
+            torch.cuda.synchronize()
+            eager.attend(0, qkv[:, :Hq], seqs=rows)
+    cache.check()
+    for a, b in ((cache.pool, eager.pool), (cache.table, eager.table), (cache.lens, eager.lens),
+                 (cache.refs, eager.refs)):
+        assert torch.equal(a, b)
+
+
+def test_python_and_native_calls_agree():
+    """A given output takes the Python path, none the native one: the same bits."""
+    from w4a16 import kv4_append, kv4_attention, qk_norm_rope
+
+    D, G, P, H, Hq, T = 128, 32, 32, 2, 6, 11
+    q, k, v = _qkv(T, Hq, H, D, torch.bfloat16, 3, "heads")
+    cos, sin = (x.to(DEV) for x in _rotation(64, 64))
+    w = torch.rand(D, generator=_gen(1)).bfloat16().to(DEV)
+    pos = torch.arange(T, dtype=torch.int32, device=DEV)
+    row = torch.zeros(T, dtype=torch.int32, device=DEV)
+    table = torch.tensor([[1, 0]], dtype=torch.int32, device=DEV)
+    pools = [torch.zeros(2, H, R.words(D, G, P), dtype=torch.int32, device=DEV) for _ in range(2)]
+    how = dict(q_weight=w, k_weight=w, interleaved=True)
+    a = qk_norm_rope(q, k, cos, sin, pos, **how)
+    b = qk_norm_rope(q, k, cos, sin, pos, out=tuple(torch.empty_like(x) for x in a), **how)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    qa = kv4_append(q, k, v, cos, sin, pos, pools[0], table, rows=row, group_size=G, **how)
+    qb = kv4_append(q, k, v, cos, sin, pos, pools[1], table, rows=row, group_size=G,
+                    out=torch.empty_like(qa), **how)
+    assert torch.equal(qa, qb) and torch.equal(*pools)
+    ln = torch.tensor([T], dtype=torch.int32, device=DEV)
+    st = torch.tensor([0, T], dtype=torch.int32, device=DEV)
+    for n in (dict(q_starts=st), dict(q_starts=st, window=3, causal=False, scale=0.2)):
+        ya = kv4_attention(qa, pools[0], table, ln, group_size=G, **n)
+        yb = kv4_attention(qa, pools[0], table, ln, group_size=G, out=torch.empty_like(qa), **n)
+        assert torch.equal(ya, yb)
+
+
+def test_refusals_on_the_device():
+    """What the kernels do not take is refused before anything is launched."""
+    import w4a16 as w
+
+    D, P = 128, 32
+    q = torch.zeros(2, 4, D, dtype=torch.float16, device=DEV)
+    k = torch.zeros(2, 2, D, dtype=torch.float16, device=DEV)
+    pool = torch.zeros(3, 2, R.words(D, 64, P), dtype=torch.int32, device=DEV)
+    table = torch.zeros(2, 3, dtype=torch.int32, device=DEV)
+    i32 = torch.zeros(2, dtype=torch.int32, device=DEV)
+    cos = torch.zeros(8, 32, device=DEV)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    refs = torch.zeros(3, dtype=torch.int32, device=DEV)
+    long = i32.long()
+    bad = [
+        lambda: w.kv4_attention(q.float(), pool, table, i32),
+        lambda: w.kv4_attention(q[:, :3], pool, table, i32),               # heads
+        lambda: w.kv4_attention(q, pool, table, i32, group_size=32),       # another pool
+        lambda: w.kv4_attention(q, pool, table.long(), i32),
+        lambda: w.kv4_attention(q, pool, table, long),
+        lambda: w.kv4_attention(q, pool, table, i32[:1]),
+        lambda: w.kv4_attention(q, pool, table, i32, window=-1),
+        lambda: w.kv4_attention(q, pool, table, i32, scale=0.0),
+        lambda: w.kv4_attention(q, pool, table, i32, seqs=i32[:1]),
+        lambda: w.kv4_attention(torch.cat((q, q)), pool, table, i32),      # rows
+        lambda: w.kv4_attention(q.transpose(1, 2), pool, table, i32),
+        lambda: w.kv4_attention(q, pool, table, i32, out=q.float()),
+        lambda: w.kv4_attention(q, pool.cpu(), table, i32),
+        lambda: w.kv4_append(q, k, k[:, :1], cos, cos, i32, pool, table),
+        lambda: w.kv4_append(q, k.bfloat16(), k, cos, cos, i32, pool, table),
+        lambda: w.kv4_append(q, k, k, cos, cos[:4], i32, pool, table),
+        lambda: w.kv4_append(q, k, k, cos.half(), cos, i32, pool, table),
+        lambda: w.kv4_append(q, k, k, cos, cos, long, pool, table),
+        lambda: w.kv4_append(q, k, k, cos, cos, i32, pool[:, :1].contiguous(), table),
+        lambda: w.kv4_append(q, k, k, cos, cos, i32, pool, table, rows=i32[:1]),
+        lambda: w.kv4_append(q, k, k, cos, cos, i32, pool, table, q_weight=cos[0]),
+        lambda: w.qk_norm_rope(q, k, cos[:, :5].contiguous(), cos[:, :5].contiguous(), i32),
+        lambda: w.kv4_read(pool, table, i32, head_dim=D, dtype=torch.float32),
+        lambda: w.kv4_read(pool, table, i32, head_dim=256),
+        lambda: w.kv4_fork(pool, table, i32, refs[:2], i32, i32, page_size=P, status=status),
+        lambda: w.kv4_fork(pool, table, i32, refs, i32, i32[:1], page_size=P, status=status),
+        lambda: w.kv4_fork(pool, table, i32, refs, i32, i32, page_size=P, status=long[:1]),
+        lambda: w.kv4_extend(table, i32, refs, i32, i32, page_size=48, status=status),
+        lambda: w.kv4_free(table, i32, refs, long),
+        lambda: w.kv4_compact(pool, table, refs[:2]),
+        lambda: w.kv4_copy_pages(pool[:, :, :-4], i32, i32),
+        lambda: w.kv4_copy_pages(pool, i32, i32[:1]),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises((AssertionError, RuntimeError)):
+            call()
+            print("not refused:", i)
+    # nothing of no tokens or no sequences is an error
+    none = q[:0]
+    assert w.kv4_attention(none, pool, table, i32).shape == (0, 4, D)
+    assert w.kv4_append(none, k[:0], k[:0], cos, cos, i32[:0], pool, table).shape == (0, 4, D)
+    assert w.kv4_read(pool, table, i32[:0], head_dim=D)[0].shape == (0, 2, D)
+    w.kv4_free(table, i32, refs, i32[:0])
+    w.kv4_copy_pages(pool, i32[:0], i32[:0])

@@ -1,23 +1,27 @@
 // Attention over the 4-bit paged cache (format: kv4_device.h).
 //
 // For a query row r (one query token and head) and a stored token t with groups g:
-//   q . k_t       = sum_g  s_tg (q_g . code_tg - 8 Q_g) + c_tg Q_g,  Q_g = sum of q_g
-//   sum_t p_t v_t = sum_t (p_t s_tg) (code_tg - 8) + sum_t p_t c_tg
-// so the matrix cores multiply the codes themselves.  For keys a masked code word is
-// a pair of subnormal halves, code * 2^-24 (16 code * 2^-24 in its odd pairs, taken
-// out of the queries), which the matrix cores multiply exactly: five bitwise
-// instructions a word of eight codes, no conversion.  Queries are scaled by a power
-// of two into the top of fp16's range (exact), the -8 is the products' initial
-// value.  The sum of subnormal products is kept on a grid of 2^-24 of (the largest
-// query value of the step * 2^-14), that is 2^-14 of a code step times a query value:
-// a score is off by at most 2^-19 of what its terms could make it, far below the
-// rounding of the weights.  (Values do not go this way: there the same grid, which
-// rounds down, moved results of one-token weights by 5e-5 of a value's range.)  For
-// values a masked word with an exponent or-ed in is 1024 + code or 64 + code, and one
-// packed subtraction makes it code - 8, exactly: nine instructions a word.
+//   q . k_t       = sum_g  s_tg (q_g . code_tg) + (c_tg - 8 s_tg) Q_g,  Q_g = sum of q_g
+//   sum_t p_t v_t = sum_t w_tg code_tg - 8 sum_t w_tg + sum_t p_t c_tg,  w_tg = p_t s_tg
+// so the matrix cores multiply the codes themselves, as subnormal halves, which they
+// multiply exactly: masking a word unpacks it.
+//   Keys: code * 2^-24, 16 code * 2^-24 in a word's odd pairs (taken out of the
+// queries), five bitwise instructions a word of eight codes.  Queries are scaled by a
+// power of two into the top of fp16's range (exact).  A token's group words are scale
+// and centre side by side, so that the second term is one product more with -8 Q and
+// Q in two halves each.
+//   Values: 16 code * 2^-24, seven instructions a word; the sum of w is a product
+// with ones, so that it is the sum of what was multiplied.
+// Sums of subnormal products are kept on a grid of 2^-24 of the largest w * 2^-14:
+// 2^-18 of a code step for values (one of 2^-14, code * 2^-24, moved results of
+// one-token weights by 5e-5 of a value's range), for keys 2^-14 of a step times a query
+// value, so that a score is off by at most 2^-19 of what its terms could make it; the
+// two halves of Q stop at 2^-15 of the largest query value.  All are far below the
+// rounding of the weights.  (Codes less 8 as normal halves, nine instructions a word,
+// and the centres' scores as fma: two prompts 289 us, this 271.)
 //
 // The weights p s of the values are rounded to fp16 (to nearest), the only rounding
-// below 32 bits; it acts on code - 8, the centres' sum stays in fp32.  The reference
+// below 32 bits; -8 sum w makes it act on code - 8, the centres' sum stays in fp32.  The reference
 // that the scores' exponents are taken against is the running maximum plus E - 7, E
 // the exponent of the largest value scale met so far: weights end below 2^15, and
 // fp16 holds each down to 2^-29 of the largest to its full precision.  Scores,
@@ -33,11 +37,12 @@
 // What bounds it: one token a sequence, memory (46 sequences of 1 to 8192 tokens, 32 /
 // 8 heads of 128, 224 MB: 58 us, 3.9 TB/s; three of 31000 to 131071, 64 / 8 heads, 265
 // MB: 58 us, 4.6 TB/s; one of 1000: 6 us, the latency of a few dependent reads);
-// prompts, the issue of vector instructions (2048 queries on 4000 tokens and 1266 on
-// 2472: 287 us, 480 TFLOP/s, vector units busy 68 % of the time, matrix cores 19 %;
-// 2048 on 16384: 570 TFLOP/s).  Of its about 370 vector instructions for 32 tokens and
-// 32 rows, unpacking takes 110, scores 64, weights and the centres' sums 80; fma with
-// an fp16 operand, packed fp16 and conversions cost 1.6 times a plain fp32 one.
+// prompts, vector and matrix instructions together, which hardly overlap on a SIMD
+// (16x16x32 products with four fma each take 10.5 ns among four waves, alone 7.0 and
+// 4.7): 2048 queries on 4000 tokens and 1266 on 2472 take 271 us, 510 TFLOP/s.  Placing
+// products between other columns' scores, weights or centres' sums changed nothing.
+// fma with an fp16 operand, packed fp16 and conversions cost 1.6 times a plain fp32
+// instruction.
 //
 // Rows whose tokens are all hidden keep a denominator of 0 and become zeros.
 // Hidden tokens, and what lies behind the last one in a page, may hold anything:
@@ -123,14 +128,11 @@ __device__ __forceinline__ f16x8 code_halves(uint32_t w) {
   const u32x4 u = {w & 0x000F000Fu, w & 0x00F000F0u, t & 0x000F000Fu, t & 0x00F000F0u};
   return __builtin_bit_cast(f16x8, u);
 }
-// Eight codes less 8.  `mg`: the two exponents (make_magic).
-__device__ __forceinline__ f16x8 value_halves(uint32_t w, const MagicRegs& mg) {
-  const uint32_t t = w >> 8;
-  const f16x2 a = {(f16)1032.0f, (f16)1032.0f}, b = {(f16)72.0f, (f16)72.0f};
-  const u32x4 u = {as_u32(as_h2(and_or(w, 0x000F000Fu, mg.m1024)) - a),
-                   as_u32(as_h2(and_or(w, 0x00F000F0u, mg.m64)) - b),
-                   as_u32(as_h2(and_or(t, 0x000F000Fu, mg.m1024)) - a),
-                   as_u32(as_h2(and_or(t, 0x00F000F0u, mg.m64)) - b)};
+// Eight codes as halves, code * 2^-20: at the top of the subnormals, so that the
+// grid of their products is 2^-18 of a code step.
+__device__ __forceinline__ f16x8 value_halves(uint32_t w) {
+  const u32x4 u = {(w << 4) & 0x00F000F0u, w & 0x00F000F0u, (w >> 4) & 0x00F000F0u,
+                   (w >> 8) & 0x00F000F0u};
   return __builtin_bit_cast(f16x8, u);
 }
 __device__ __forceinline__ float lo_f32(uint32_t w) { return (float)as_h((uint16_t)w); }
@@ -198,6 +200,11 @@ struct Stage {
       for (int h = 0; h < D / 128; ++h) read4(lds + 256 * (j * (D / 128) + h) + 4 * lane, w + 4 * h);
     }
   }
+  // (the group word of the token that the lane's key words of tile j belong to)
+  static __device__ __forceinline__ uint32_t tile_group(const uint32_t* lds, int n, int j,
+                                                        int lane) {
+    return lds[kGroups + 64 * n + 8 * ((lane & 15) >> 2) + 4 * j + (lane & 3)];
+  }
   static __device__ __forceinline__ void values(const uint32_t* lds, int h, int lane,
                                                 uint32_t w[4]) {
     read4(lds + 256 * (kCodeLoads + h) + 4 * lane, w);
@@ -226,18 +233,45 @@ __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
+// (c - 8 s) Q of all groups for a tile's scores: a token's group words, which are pairs
+// of scale and centre, times pairs of -8 Q and Q.  Lanes 0-15 hold these rounded to
+// fp16, lanes 16-31 what is left of them (to 2^-25, 2^-15 of the largest query value).
+template <int NG>
+struct GroupTerms {
+  static constexpr int kWords = NG == 4 ? 4 : 2;
+  typedef uint32_t A __attribute__((ext_vector_type(kWords)));
+  typedef f16 B __attribute__((ext_vector_type(2 * kWords)));
+  static __device__ __forceinline__ void set(B& b, int n, float Q, int lane) {
+    if (n == 0) b = B{};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float x = i ? Q : -8.0f * Q;
+      const f16 hi = (f16)x;
+      b[2 * n + i] = lane < 16 ? hi : lane < 32 ? (f16)(x - (float)hi) : (f16)0.0f;
+    }
+  }
+  static __device__ __forceinline__ f32x4 product(A a, B b) {
+    const f32x4 z = {0, 0, 0, 0};
+    if constexpr (NG == 4)
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(B, a), b, z, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(B, a), b, z, 0, 0, 0);
+  }
+};
+
 template <int D, int NG, int C>
 struct AttnWave {
+  typedef GroupTerms<NG> Terms;
   static constexpr int kSteps = D / 32, kTiles = D / 16;
   f16x8 q[C][kSteps];
-  float Q[C][NG];              // sums of the scaled queries, 2^-24
+  typename Terms::B terms[C];           // -8 Q and Q of every group, 2^-24, by two halves
   float fac[C];                // score in powers of two = x * fac
   int see_lo[C], see_hi[C];    // tokens that the lane's row sees
-  f32x4 acc[C][kTiles];
+  f32x4 acc[C][kTiles];        // sums of w code, 2^-20
+  f32x4 wsum[C][NG];           // sums of w, four times
   float ref[C], l[C], csum[C][NG];   // the reference; sums of p and p c
   int E;
   uint16_t limit;   // 2^E as fp16: scales from this on move the reference
-  MagicRegs mg;
 
   __device__ __forceinline__ void start() {
 #pragma unroll
@@ -245,13 +279,15 @@ struct AttnWave {
 #pragma unroll
       for (int i = 0; i < kTiles; ++i) acc[c][i] = f32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int n = 0; n < NG; ++n) csum[c][n] = 0.0f;
+      for (int n = 0; n < NG; ++n) {
+        csum[c][n] = 0.0f;
+        wsum[c][n] = f32x4{0, 0, 0, 0};
+      }
       ref[c] = kNoScore;
       l[c] = 0.0f;
     }
     E = -24;
     limit = 1;
-    mg = make_magic();
   }
 
   // Row `r` of the lane, as it lies in memory; rows past the tile's queries see
@@ -272,7 +308,7 @@ struct AttnWave {
   // The rows as the first product takes them: 2^e brings a row's largest value into
   // [2^14, 2^15).
   template <bool BF16>
-  __device__ __forceinline__ void convert(float scale_log2) {
+  __device__ __forceinline__ void convert(float scale_log2, int lane) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       u32x4 x[kSteps];
@@ -293,26 +329,27 @@ struct AttnWave {
       // (a subnormal bf16 needs more than fp32's largest power of two: it stays small)
       e = min(e, 127);
       const float up = ldexpf(1.0f, e), up16 = ldexpf(1.0f, e - 4);
+      float Q[NG];
 #pragma unroll
-      for (int n = 0; n < NG; ++n) Q[c][n] = 0.0f;
+      for (int n = 0; n < NG; ++n) Q[n] = 0.0f;
 #pragma unroll
       for (int k = 0; k < kSteps; ++k)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float y = to_f32<BF16>((uint16_t)(x[k][j / 2] >> (16 * (j & 1))));
-          Q[c][k / (kSteps / NG)] = fmaf(y, up, Q[c][k / (kSteps / NG)]);
+          Q[k / (kSteps / NG)] = fmaf(y, up, Q[k / (kSteps / NG)]);
           q[c][k][j] = (f16)(y * (j & 2 ? up16 : up));
         }
 #pragma unroll
-      for (int n = 0; n < NG; ++n) Q[c][n] = sum_rows(Q[c][n]) * 0x1p-24f;
+      for (int n = 0; n < NG; ++n) Terms::set(terms[c], n, sum_rows(Q[n]) * 0x1p-24f, lane);
       fac[c] = ldexpf(scale_log2, 24 - e);
     }
   }
-  __device__ __forceinline__ void convert(const AttnArgs& a) {
+  __device__ __forceinline__ void convert(const AttnArgs& a, int lane) {
     if (a.bf16)
-      convert<true>(a.scale_log2);
+      convert<true>(a.scale_log2, lane);
     else
-      convert<false>(a.scale_log2);
+      convert<false>(a.scale_log2, lane);
   }
 
   // 32 tokens from t on.  `mask`: some of them are hidden from some row.
@@ -327,17 +364,19 @@ struct AttnWave {
     for (int j = 0; j < 2; ++j) S::keys(lds, j, lane, kw[j]);
 #pragma unroll
     for (int n = 0; n < NG; ++n) S::key_groups(lds, n, lane, kg[n]);
+    typename Terms::A kt[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < Terms::kWords; ++i) kt[j][i] = S::tile_group(lds, i < NG ? i : 0, j, lane);
     __builtin_amdgcn_sched_barrier(0);
-    f32x4 s[2][C][NG];
+    f32x4 s[2][C][NG], u[2][C];   // products of codes; -8 s Q + c Q of all groups
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int n = 0; n < NG; ++n) {
-          const float z = -8.0f * Q[c][n];
-          s[j][c][n] = f32x4{z, z, z, z};
-        }
+        for (int n = 0; n < NG; ++n) s[j][c][n] = f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int k = 0; k < kSteps; ++k) {
         const f16x8 w = code_halves(kw[j][k]);
@@ -346,6 +385,8 @@ struct AttnWave {
           s[j][c][k / (kSteps / NG)] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
               w, q[c][k], s[j][c][k / (kSteps / NG)], 0, 0, 0);
       }
+#pragma unroll
+      for (int c = 0; c < C; ++c) u[j][c] = Terms::product(kt[j], terms[c]);
     }
 #pragma unroll
     for (int n = 0; n < NG; ++n) S::value_groups(lds, n, lane, vg[n]);
@@ -357,14 +398,7 @@ struct AttnWave {
       for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          sc[c][i] = fmaf(hi_f32(kg[n][i]), Q[c][n], n ? sc[c][i] : 0.0f);
-          asm volatile("" : "+v"(sc[c][i]));
-        }
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          sc[c][i] = fmaf(lo_f32(kg[n][i]), s[i / 4][c][n][i % 4], sc[c][i]);
+          sc[c][i] = fmaf(lo_f32(kg[n][i]), s[i / 4][c][n][i % 4], n ? sc[c][i] : u[i / 4][c][i % 4]);
           asm volatile("" : "+v"(sc[c][i]));
         }
     }
@@ -428,7 +462,10 @@ struct AttnWave {
         ref[c] = to;
         l[c] *= alpha;
 #pragma unroll
-        for (int n = 0; n < NG; ++n) csum[c][n] *= alpha;
+        for (int n = 0; n < NG; ++n) {
+          csum[c][n] *= alpha;
+          wsum[c][n] *= alpha;
+        }
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) acc[c][i] *= alpha;
       }
@@ -461,13 +498,23 @@ struct AttnWave {
         for (int i = 0; i < 8; ++i)
 #pragma unroll
           for (int n = 0; n < NG; ++n) {
-            w[c][n][i] = (f16)fmaf(sc[c][i], lo_f32(vg[n][i]), 0.0f);
+            // (an fma and a conversion take less time than the one that does both)
+            float x = fmaf(sc[c][i], lo_f32(vg[n][i]), 0.0f);
+            asm volatile("" : "+v"(x));
+            w[c][n][i] = (f16)x;
             csum[c][n] = fmaf(sc[c][i], hi_f32(vg[n][i]), csum[c][n]);
           }
     }
+    const f16 one = (f16)1.0f;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+        wsum[c][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+            f16x8{one, one, one, one, one, one, one, one}, w[c][n], wsum[c][n], 0, 0, 0);
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) {
-      const f16x8 v = value_halves(vw[i], mg);
+      const f16x8 v = value_halves(vw[i]);
 #pragma unroll
       for (int c = 0; c < C; ++c)
         acc[c][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[c][i / (kTiles / NG)], acc[c][i],
@@ -493,12 +540,12 @@ struct AttnWave {
     for (int c = 0; c < C; ++c) {
       l[c] = sum_rows(l[c]);
 #pragma unroll
-      for (int n = 0; n < NG; ++n) csum[c][n] = sum_rows(csum[c][n]);
+      for (int n = 0; n < NG; ++n) csum[c][n] = fmaf(-8.0f, wsum[c][n][0], sum_rows(csum[c][n]));
 #pragma unroll
       for (int i = 0; i < kTiles; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          acc[c][i][j] += csum[c][i / (kTiles / NG)];
+          acc[c][i][j] = fmaf(acc[c][i][j], 0x1p20f, csum[c][i / (kTiles / NG)]);
     }
   }
 };
@@ -628,7 +675,7 @@ kv4_attention_kernel(const AttnArgs a) {
 #pragma unroll
     for (int i = 0; i < kS - 1; ++i)
       if (next < end) fill(i);
-    w.convert(a);
+    w.convert(a, lane);
     int slot = 0;
     for (int kb = first + wave; kb < end; kb += kShare) {
       const int last = slot == 0 ? kS - 1 : slot - 1;

@@ -15,10 +15,9 @@
 // Sums of subnormal products are kept on a grid of 2^-24 of the largest w * 2^-14:
 // 2^-18 of a code step for values (one of 2^-14, code * 2^-24, moved results of
 // one-token weights by 5e-5 of a value's range), for keys 2^-14 of a step times a query
-// value, so that a score is off by at most 2^-19 of what its terms could make it; the
-// two halves of Q stop at 2^-15 of the largest query value.  All are far below the
-// rounding of the weights.  (Codes less 8 as normal halves, nine instructions a word,
-// and the centres' scores as fma: two prompts 289 us, this 271.)
+// value, so that a score is off by at most 2^-19 of what its terms could make it; both
+// are far below the rounding of the weights.  (Codes less 8 as normal halves, nine
+// instructions a word, and the centres' scores as fma: two prompts 289 us, this 271.)
 //
 // The weights p s of the values are rounded to fp16 (to nearest), the only rounding
 // below 32 bits; -8 sum w makes it act on code - 8, the centres' sum stays in fp32.  The reference
@@ -235,7 +234,8 @@ __device__ __forceinline__ void wait_loads() {
 
 // (c - 8 s) Q of all groups for a tile's scores: a token's group words, which are pairs
 // of scale and centre, times pairs of -8 Q and Q.  Lanes 0-15 hold these rounded to
-// fp16, lanes 16-31 what is left of them (to 2^-25, 2^-15 of the largest query value).
+// fp16, lanes 16-31 what is left of them times 2^10, and 2^-10 of the words: together
+// they are Q to 2^-35, 2^-25 of the largest query value.
 template <int NG>
 struct GroupTerms {
   static constexpr int kWords = NG == 4 ? 4 : 2;
@@ -247,8 +247,12 @@ struct GroupTerms {
     for (int i = 0; i < 2; ++i) {
       const float x = i ? Q : -8.0f * Q;
       const f16 hi = (f16)x;
-      b[2 * n + i] = lane < 16 ? hi : lane < 32 ? (f16)(x - (float)hi) : (f16)0.0f;
+      b[2 * n + i] = lane < 16 ? hi : lane < 32 ? (f16)((x - (float)hi) * 0x1p10f) : (f16)0.0f;
     }
+  }
+  static __device__ __forceinline__ f16x2 part(int lane) {
+    const f16 x = lane < 16 ? (f16)1.0f : (f16)0x1p-10f;
+    return f16x2{x, x};
   }
   static __device__ __forceinline__ f32x4 product(A a, B b) {
     const f32x4 z = {0, 0, 0, 0};
@@ -264,6 +268,7 @@ struct AttnWave {
   typedef GroupTerms<NG> Terms;
   static constexpr int kSteps = D / 32, kTiles = D / 16;
   f16x8 q[C][kSteps];
+  f16x2 part;                  // of the group words that the lane's terms take
   typename Terms::B terms[C];           // -8 Q and Q of every group, 2^-24, by two halves
   float fac[C];                // score in powers of two = x * fac
   int see_lo[C], see_hi[C];    // tokens that the lane's row sees
@@ -273,7 +278,7 @@ struct AttnWave {
   int E;
   uint16_t limit;   // 2^E as fp16: scales from this on move the reference
 
-  __device__ __forceinline__ void start() {
+  __device__ __forceinline__ void start(int lane) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
 #pragma unroll
@@ -286,6 +291,7 @@ struct AttnWave {
       ref[c] = kNoScore;
       l[c] = 0.0f;
     }
+    part = Terms::part(lane);
     E = -24;
     limit = 1;
   }
@@ -385,6 +391,8 @@ struct AttnWave {
           s[j][c][k / (kSteps / NG)] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
               w, q[c][k], s[j][c][k / (kSteps / NG)], 0, 0, 0);
       }
+#pragma unroll
+      for (int i = 0; i < Terms::kWords; ++i) kt[j][i] = as_u32(as_h2(kt[j][i]) * part);
 #pragma unroll
       for (int c = 0; c < C; ++c) u[j][c] = Terms::product(kt[j], terms[c]);
     }
@@ -644,7 +652,7 @@ kv4_attention_kernel(const AttnArgs a) {
   w.any_hi = a.causal ? min(max(p1 + 1, 0), s.n) : s.n;
   w.any_lo = a.window > 0 ? min(max(0, p0 - a.window + 1), w.any_hi) : 0;
   w.all_lo = a.window > 0 ? max(0, p1 - a.window + 1) : 0;
-  w.start();
+  w.start(lane);
   {
     // the split's blocks
     const int first = s.first + split * a.chunk;

@@ -422,6 +422,26 @@ def test_attention_any_size_of_query(size):
     _check_attention(q, pool, table, [n], D, G, P, out, scale=scale, what=str(size))
 
 
+@pytest.mark.parametrize("shape", SHAPES[:4], ids=lambda c: "-".join(map(str, c)))
+def test_attention_one_large_query_value(shape):
+    """A query value far above the others leaves the others' products their precision:
+    scores of single tokens (lse) and of many."""
+    from w4a16 import kv4_attention
+
+    D, G, P, Hq, H, dtype = shape
+    lens = [1] * 40 + [500]
+    pages = 41 + -(-500 // P)
+    table = _tables(len(lens), -(-500 // P), pages, lens, P, 31)
+    pool = _random_pool(pages, H, D, G, P, 32)
+    q = torch.randn(len(lens), Hq, D, generator=_gen(33))
+    q[:, :, 5::32] = 64.0
+    q = q.to(dtype)
+    out, lse = kv4_attention(q.to(DEV), pool.to(DEV), table.to(DEV),
+                             torch.tensor(lens, dtype=torch.int32, device=DEV), group_size=G,
+                             return_lse=True)
+    _check_attention(q, pool, table, lens, D, G, P, out, lse, what="one large")
+
+
 def _nan_meta(pool, D, G, P, page, tokens):
     """NaN and infinite scales and centres at tokens of a page (all heads)."""
     NG, a, c = D // G, P * D // 8, P * D // 4 + (D // G) * P

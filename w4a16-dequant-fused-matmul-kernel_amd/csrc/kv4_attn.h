@@ -4,26 +4,24 @@
 //   q . k_t       = sum_g  s_tg (q_g . code_tg) + (c_tg - 8 s_tg) Q_g,  Q_g = sum of q_g
 //   sum_t p_t v_t = sum_t w_tg code_tg - 8 sum_t w_tg + sum_t p_t c_tg,  w_tg = p_t s_tg
 // so the matrix cores multiply the codes themselves, as subnormal halves, which they
-// multiply exactly: masking a word unpacks it.
-//   Keys: code * 2^-24, 16 code * 2^-24 in a word's odd pairs (taken out of the
-// queries), five bitwise instructions a word of eight codes.  Queries are scaled by a
-// power of two into the top of fp16's range (exact).  A token's group words are scale
-// and centre side by side, so that the second term is one product more with -8 Q and
-// Q in two halves each.
-//   Values: 16 code * 2^-24, seven instructions a word; the sum of w is a product
-// with ones, so that it is the sum of what was multiplied.
-// Sums of subnormal products are kept on a grid of 2^-24 of the largest w * 2^-14:
-// 2^-18 of a code step for values (one of 2^-14, code * 2^-24, moved results of
-// one-token weights by 5e-5 of a value's range), for keys 2^-14 of a step times a query
-// value, so that a score is off by at most 2^-19 of what its terms could make it; both
-// are far below the rounding of the weights.  (Codes less 8 as normal halves, nine
-// instructions a word, and the centres' scores as fma: two prompts 289 us, this 271.)
+// multiply exactly: a word is unpacked by masks and shifts alone, seven instructions
+// for eight codes.  Queries are scaled by a power of two into the top of fp16's range
+// (exact).  A token's group words are scale and centre side by side, so that the second
+// term is one product more with -8 Q and Q in two halves each.  The sum of w is a
+// product with ones, so that it is the sum of what was multiplied.
+//   Products with a subnormal operand are added on a grid: 2^-24 of the largest other
+// operand of the 32 times 2^-14, each rounded down to it.  The codes stand at 2^-20, so
+// that this is 2^-18 of a code step, times the largest query value or weight of the
+// 32, for those that are much smaller.  (At 2^-24 keys take five instructions, and two
+// prompts 270 us for 278; but one query value 64 times the others moved scores by 4e-4,
+// now by 1e-5, and one-token weights moved results by 5e-5 of a value's range.  Codes
+// less 8 as normal halves for values, and the centres' scores as fma: 289 us.)
 //
 // The weights p s of the values are rounded to fp16 (to nearest), the only rounding
-// below 32 bits; -8 sum w makes it act on code - 8, the centres' sum stays in fp32.  The reference
-// that the scores' exponents are taken against is the running maximum plus E - 7, E
-// the exponent of the largest value scale met so far: weights end below 2^15, and
-// fp16 holds each down to 2^-29 of the largest to its full precision.  Scores,
+// below 32 bits; -8 sum w makes it act on code - 8, the centres' sum stays in fp32.  The
+// reference that the scores' exponents are taken against is the running maximum plus
+// E - 7, E the exponent of the largest value scale met so far: weights end below 2^15,
+// and fp16 holds each down to 2^-29 of the largest to its full precision.  Scores,
 // references, denominators and all sums are fp32.
 //
 // A wave has 16 * C query rows and takes 32 tokens at a time: tokens are the rows
@@ -38,7 +36,7 @@
 // MB: 58 us, 4.6 TB/s; one of 1000: 6 us, the latency of a few dependent reads);
 // prompts, vector and matrix instructions together, which hardly overlap on a SIMD
 // (16x16x32 products with four fma each take 10.5 ns among four waves, alone 7.0 and
-// 4.7): 2048 queries on 4000 tokens and 1266 on 2472 take 271 us, 510 TFLOP/s.  Placing
+// 4.7): 2048 queries on 4000 tokens and 1266 on 2472 take 278 us, 496 TFLOP/s.  Placing
 // products between other columns' scores, weights or centres' sums changed nothing.
 // fma with an fp16 operand, packed fp16 and conversions cost 1.6 times a plain fp32
 // instruction.
@@ -121,15 +119,8 @@ __device__ __forceinline__ float sum_rows(float v) {
   return over_rows(v, [](float a, float b) { return a + b; });
 }
 
-// Eight codes as halves: code * 2^-24 at 0, 1, 4, 5, 16 * code * 2^-24 at 2, 3, 6, 7.
+// Eight codes as subnormal halves, code * 2^-20.
 __device__ __forceinline__ f16x8 code_halves(uint32_t w) {
-  const uint32_t t = w >> 8;
-  const u32x4 u = {w & 0x000F000Fu, w & 0x00F000F0u, t & 0x000F000Fu, t & 0x00F000F0u};
-  return __builtin_bit_cast(f16x8, u);
-}
-// Eight codes as halves, code * 2^-20: at the top of the subnormals, so that the
-// grid of their products is 2^-18 of a code step.
-__device__ __forceinline__ f16x8 value_halves(uint32_t w) {
   const u32x4 u = {(w << 4) & 0x00F000F0u, w & 0x00F000F0u, (w >> 4) & 0x00F000F0u,
                    (w >> 8) & 0x00F000F0u};
   return __builtin_bit_cast(f16x8, u);
@@ -235,7 +226,7 @@ __device__ __forceinline__ void wait_loads() {
 // (c - 8 s) Q of all groups for a tile's scores: a token's group words, which are pairs
 // of scale and centre, times pairs of -8 Q and Q.  Lanes 0-15 hold these rounded to
 // fp16, lanes 16-31 what is left of them times 2^10, and 2^-10 of the words: together
-// they are Q to 2^-35, 2^-25 of the largest query value.
+// they are Q to 2^-35, 2^-29 of the largest query value.
 template <int NG>
 struct GroupTerms {
   static constexpr int kWords = NG == 4 ? 4 : 2;
@@ -269,7 +260,7 @@ struct AttnWave {
   static constexpr int kSteps = D / 32, kTiles = D / 16;
   f16x8 q[C][kSteps];
   f16x2 part;                  // of the group words that the lane's terms take
-  typename Terms::B terms[C];           // -8 Q and Q of every group, 2^-24, by two halves
+  typename Terms::B terms[C];           // -8 Q and Q of every group, 2^-20, by two halves
   float fac[C];                // score in powers of two = x * fac
   int see_lo[C], see_hi[C];    // tokens that the lane's row sees
   f32x4 acc[C][kTiles];        // sums of w code, 2^-20
@@ -334,7 +325,7 @@ struct AttnWave {
       if (most > 0.0f && most < __builtin_inff()) e = 15 - __builtin_amdgcn_frexp_expf(most);
       // (a subnormal bf16 needs more than fp32's largest power of two: it stays small)
       e = min(e, 127);
-      const float up = ldexpf(1.0f, e), up16 = ldexpf(1.0f, e - 4);
+      const float up = ldexpf(1.0f, e);
       float Q[NG];
 #pragma unroll
       for (int n = 0; n < NG; ++n) Q[n] = 0.0f;
@@ -344,11 +335,11 @@ struct AttnWave {
         for (int j = 0; j < 8; ++j) {
           const float y = to_f32<BF16>((uint16_t)(x[k][j / 2] >> (16 * (j & 1))));
           Q[k / (kSteps / NG)] = fmaf(y, up, Q[k / (kSteps / NG)]);
-          q[c][k][j] = (f16)(y * (j & 2 ? up16 : up));
+          q[c][k][j] = (f16)(y * up);
         }
 #pragma unroll
-      for (int n = 0; n < NG; ++n) Terms::set(terms[c], n, sum_rows(Q[n]) * 0x1p-24f, lane);
-      fac[c] = ldexpf(scale_log2, 24 - e);
+      for (int n = 0; n < NG; ++n) Terms::set(terms[c], n, sum_rows(Q[n]) * 0x1p-20f, lane);
+      fac[c] = ldexpf(scale_log2, 20 - e);
     }
   }
   __device__ __forceinline__ void convert(const AttnArgs& a, int lane) {
@@ -522,7 +513,7 @@ struct AttnWave {
             f16x8{one, one, one, one, one, one, one, one}, w[c][n], wsum[c][n], 0, 0, 0);
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) {
-      const f16x8 v = value_halves(vw[i]);
+      const f16x8 v = code_halves(vw[i]);
 #pragma unroll
       for (int c = 0; c < C; ++c)
         acc[c][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[c][i / (kTiles / NG)], acc[c][i],

@@ -366,6 +366,35 @@ def test_attention_many_tokens(shape, causal, window):
                          causal=causal, window=window, what=f"few {max_q}")
 
 
+@pytest.mark.parametrize("nq", [1, 4])
+@pytest.mark.parametrize("D,G,dtype", [(128, 128, torch.float16), (128, 64, torch.bfloat16),
+                                       (128, 32, torch.float16), (64, 64, torch.bfloat16),
+                                       (64, 32, torch.float16)])
+def test_attention_few_blocks_for_eight_waves(D, G, dtype, nq):
+    """Contexts of 17 blocks and a few more, which one workgroup takes whole, and rows
+    shorter and longer than was said."""
+    from w4a16 import kv4_attention
+
+    P, Hq, H = 64, 8, 2
+    said = 560 if D == 128 else 1100
+    lens = [said, 4, 33, 257, said + 300, 512]
+    pages = sum(-(-n // P) for n in lens)
+    table = _tables(len(lens), max(-(-n // P) for n in lens), pages, lens, P, 41)
+    pool = _random_pool(pages, H, D, G, P, 42)
+    T = nq * len(lens)
+    q = (torch.randn(T, Hq, D, generator=_gen(43)) * 2).to(dtype)
+    starts = list(range(0, T + 1, nq))
+    dev = [x.to(DEV) for x in (q, pool, table, torch.tensor(lens, dtype=torch.int32))]
+    how = dict(q_starts=torch.tensor(starts, dtype=torch.int32, device=DEV), max_q=nq) if nq > 1 else {}
+    for window in (0, 530):
+        out, lse = kv4_attention(*dev, group_size=G, max_context=said, window=window,
+                                 return_lse=True, **how)
+        _check_attention(q, pool, table, lens, D, G, P, out, lse, starts, window=window,
+                         what=f"window {window}")
+        again = kv4_attention(*dev, group_size=G, max_context=said, window=window, **how)
+        assert torch.equal(out, again)
+
+
 @pytest.mark.parametrize("D,G,Hq,H,nq", [(128, 64, 4, 1, 1), (64, 64, 2, 2, 40), (256, 64, 6, 2, 5)])
 def test_attention_long_and_split(D, G, Hq, H, nq):
     """A context over which the work is split, value scales of very unlike sizes."""

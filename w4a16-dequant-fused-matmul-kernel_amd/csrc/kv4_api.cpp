@@ -152,6 +152,7 @@ int w4a16_kv4_attention(const w4a16_kv4* kv, const w4a16_kv4_query* q, void* wor
   if (p.workspace && (!workspace || workspace_bytes < p.workspace)) return W4A16_ERR_WORKSPACE;
   if (p.workspace && !aligned(workspace, 256)) return W4A16_ERR_BAD_PLAN;
   a.rows_form = p.rows_form;
+  a.wide = p.wide;
   a.cols = p.cols;
   a.tiles = p.tiles;
   a.splits = p.splits;

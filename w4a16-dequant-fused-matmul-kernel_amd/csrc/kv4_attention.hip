@@ -7,6 +7,7 @@ namespace {
 
 // Most splits of a call, and the most that one group of lanes joins by itself.
 constexpr int kMaxSplits = 256, kFewSplits = 8;
+constexpr int kJoinThreads = 256;
 
 // Joins the splits of a query row; D / 4 lanes to a split, 16 bytes to a lane.
 // kMany: a workgroup takes one row and 1024 / D splits at a time, its weights worked
@@ -15,9 +16,9 @@ constexpr int kMaxSplits = 256, kFewSplits = 8;
 // its own.  Bounded by the launch and two dependent reads where rows are few, by
 // memory where they are many.
 template <int D, bool kMany>
-__global__ __launch_bounds__(kAttnThreads) void kv4_join_kernel(const AttnArgs a, int tile_rows,
+__global__ __launch_bounds__(kJoinThreads) void kv4_join_kernel(const AttnArgs a, int tile_rows,
                                                                 int max_rows) {
-  constexpr int kLanes = D / 4, kGroups = kAttnThreads / kLanes;
+  constexpr int kLanes = D / 4, kGroups = kJoinThreads / kLanes;
   __shared__ f32x4 sum[kMany ? kGroups : 1][kLanes];
   __shared__ float weight[kMany ? kMaxSplits : 1], most[4], den[4];
   const int at = threadIdx.x % kLanes, o = threadIdx.x / kLanes;
@@ -87,12 +88,12 @@ __global__ __launch_bounds__(kAttnThreads) void kv4_join_kernel(const AttnArgs a
 template <int D>
 void launch_join(const AttnArgs& a, int tile_rows, int max_rows, hipStream_t st) {
   if (a.splits > kFewSplits) {
-    kv4_join_kernel<D, true><<<dim3((unsigned)a.heads * max_rows * a.batch), kAttnThreads, 0, st>>>(
+    kv4_join_kernel<D, true><<<dim3((unsigned)a.heads * max_rows * a.batch), kJoinThreads, 0, st>>>(
         a, tile_rows, max_rows);
   } else {
-    constexpr int kGroups = kAttnThreads / (D / 4);
+    constexpr int kGroups = kJoinThreads / (D / 4);
     kv4_join_kernel<D, false>
-        <<<dim3((unsigned)a.heads * ((max_rows + kGroups - 1) / kGroups) * a.batch), kAttnThreads, 0,
+        <<<dim3((unsigned)a.heads * ((max_rows + kGroups - 1) / kGroups) * a.batch), kJoinThreads, 0,
            st>>>(a, tile_rows, max_rows);
   }
 }
@@ -121,6 +122,13 @@ Kv4Plan kv4_attention_plan(const w4a16_kv4& kv, const w4a16_kv4_query& q) {
   int64_t want = p.rows_form ? (units >= 1024 ? 1 : (2048 + units - 1) / units)
                  : blocks <= 16 ? 1
                                 : (1024 + units - 1) / units;
+  // Eight waves and no join where that leaves each few blocks, and a workgroup has a CU
+  // of its own (32 / 8 heads of 128, 500 tokens: 16 sequences 12.9 us in splits, 9.9 so;
+  // 16 heads of 64, 16 sequences of 500: 12.8, 9.1, of 1200: 15.7, 12.7; but 1000 tokens
+  // of heads of 128 12.5 either way, and 64 sequences of them 21, 23.5).
+  p.wide = p.cols == 1 && !p.rows_form && kv.head_dim < 256 && units <= 256 && blocks > 16 &&
+           blocks * kv.head_dim < 2560;
+  if (p.wide) want = 1;
   const int64_t most = (blocks + least - 1) / least;
   if (want > most) want = most;
   if (want < 1) want = 1;
@@ -169,7 +177,8 @@ hipError_t launch_kv4_attention(const Kv4Attn& c, hipStream_t st) {
   const hipError_t e = c.rows_form && D == 256 ? launch_attention_rows256(a, NG, st)
                        : c.rows_form ? launch_attention_rows(a, D, NG, st)
                        : c.cols == 2 ? launch_attention_tokens2(a, D, NG, st)
-                                     : launch_attention_tokens1(a, D, NG, st);
+                                     : c.wide ? launch_attention_tokens1_wide(a, D, NG, st)
+                                              : launch_attention_tokens1(a, D, NG, st);
   if (e != hipSuccess || c.splits == 1) return e;
   const int tile_rows = 16 * c.cols;
   const int max_rows = (int)q.max_q * a.per_kv;

@@ -51,7 +51,6 @@
 
 namespace w4a16 {
 
-constexpr int kAttnThreads = 256;   // of a workgroup whose waves share their rows
 constexpr float kNoScore = -1e30f;   // reference (a power of two) before any score
 
 struct AttnArgs {
@@ -595,23 +594,24 @@ constexpr int kWaves = C == 1 && D + 32 * NG <= 160   ? 4
                        : C == 1 && D + 32 * NG <= 192 ? 3
                        : C * (D + 32 * (NG - 1)) <= 320 ? 2 : 1;
 
-// A workgroup is four waves that share 16 * C rows and take blocks of 32 tokens in
-// turn, or (kRows) one wave that takes all of them.  (Four waves with rows of their
+// A workgroup is W waves, four or eight, that share 16 * C rows and take blocks of 32
+// tokens in turn, or one wave that takes all of them.  (Four waves with rows of their
 // own and the same buffers wait for each other and leave larger pieces: prompts of
 // 2048 and 1266 tokens 361 us, single waves 334.)  Grid: kv head fastest (an XCD
 // then keeps to few heads and finds their codes in its L2), then sequence, split,
 // and the row tiles from the last, which sees the most tokens, to the first.  (Splits
 // before sequences put the empty splits of short sequences on the same CUs: 46
 // sequences of 1 to 8192 tokens in 4 splits 85 us, in 3 65.)
-template <int D, int NG, int C, bool kRows>
-__global__ __launch_bounds__(kRows ? 64 : kAttnThreads, (kWaves<D, NG, C>)) void
+template <int D, int NG, int C, int W>
+__global__ __launch_bounds__(64 * W, (kWaves<D, NG, C>)) void
 kv4_attention_kernel(const AttnArgs a) {
   typedef Stage<D, NG> S;
-  constexpr int kTiles = D / 16, kS = kStages, kShare = kRows ? 1 : 4;
+  constexpr bool kRows = W == 1;
+  constexpr int kTiles = D / 16, kS = kStages, kShare = W;
   constexpr int kRing = kShare * kS * S::kWords;
   // the four waves' results (rows 4 floats apart beyond D: the four groups of lanes
   // use different banks), then their maxima and denominators
-  constexpr int kSumRow = D + 4, kSum = kRows ? 0 : 4 * 16 * kSumRow + 4 * 16 * 2;
+  constexpr int kSumRow = D + 4, kSum = kRows ? 0 : W * 16 * kSumRow + W * 16 * 2;
   __shared__ __attribute__((aligned(16))) uint32_t lds[kRing > kSum ? kRing : kSum];
   const int lane = threadIdx.x & 63;
   const int wave = kRows ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -724,7 +724,7 @@ kv4_attention_kernel(const AttnArgs a) {
     }
   } else {
     float (*sum)[16][kSumRow] = reinterpret_cast<float(*)[16][kSumRow]>(lds);
-    float (*ml)[16][2] = reinterpret_cast<float(*)[16][2]>(lds + 4 * 16 * kSumRow);
+    float (*ml)[16][2] = reinterpret_cast<float(*)[16][2]>(lds + W * 16 * kSumRow);
     __syncthreads();   // the buffers have been read
 #pragma unroll
     for (int c = 0; c < C; ++c) {
@@ -734,28 +734,33 @@ kv4_attention_kernel(const AttnArgs a) {
         ml[wave][col][1] = w.l[c];
       }
       __syncthreads();
-      const float m1 = fmaxf(fmaxf(ml[0][col][0], ml[1][col][0]), fmaxf(ml[2][col][0], ml[3][col][0]));
+      float m1 = ml[0][col][0];
+#pragma unroll
+      for (int o = 1; o < W; ++o) m1 = fmaxf(m1, ml[o][col][0]);
       const float mine = exp2f(w.ref[c] - m1);
 #pragma unroll
       for (int t = 0; t < kTiles; ++t)
         *reinterpret_cast<f32x4*>(&sum[wave][col][16 * t + 4 * g]) = w.acc[c][t] * mine;
       __syncthreads();
-      // sixteen threads a row, four values at a time
-      const int rr = threadIdx.x >> 4, at = threadIdx.x & 15, r = r0 + 16 * c + rr;
+      // 4 W threads a row, four values at a time
+      const int rr = threadIdx.x / (4 * W), at = threadIdx.x % (4 * W), r = r0 + 16 * c + rr;
       if (r >= R) continue;
-      const float mm = fmaxf(fmaxf(ml[0][rr][0], ml[1][rr][0]), fmaxf(ml[2][rr][0], ml[3][rr][0]));
+      float mm = ml[0][rr][0];
+#pragma unroll
+      for (int o = 1; o < W; ++o) mm = fmaxf(mm, ml[o][rr][0]);
       float l = 0.0f;
 #pragma unroll
-      for (int o = 0; o < 4; ++o) l += ml[o][rr][1] * exp2f(ml[o][rr][0] - mm);
+      for (int o = 0; o < W; ++o) l += ml[o][rr][1] * exp2f(ml[o][rr][0] - mm);
       const int i = r / a.per_kv;
       const int64_t qrow = (int64_t)(s.q0 + i) * a.q_heads + h * a.per_kv + (r - i * a.per_kv);
       const bool any = l > 0.0f || l != l;
       const float inv = any ? 1.0f / l : 0.0f;
 #pragma unroll
-      for (int d = 0; d < D; d += 64) {
+      for (int d = 0; d < D; d += 16 * W) {
+        if (16 * W > D && 4 * at >= D) break;
         f32x4 v = *reinterpret_cast<f32x4*>(&sum[0][rr][d + 4 * at]);
 #pragma unroll
-        for (int o = 1; o < 4; ++o) v += *reinterpret_cast<f32x4*>(&sum[o][rr][d + 4 * at]);
+        for (int o = 1; o < W; ++o) v += *reinterpret_cast<f32x4*>(&sum[o][rr][d + 4 * at]);
         if (a.splits > 1) {
           *reinterpret_cast<f32x4*>(part_values(a, split, qrow, D) + d + 4 * at) = v;
         } else {
@@ -779,22 +784,23 @@ kv4_attention_kernel(const AttnArgs a) {
 }
 
 // One form of the kernel for every head size and group count.
-template <int C, bool kRows>
+template <int C, int W>
 hipError_t launch_attention_form(const AttnArgs& a, int D, int NG, hipStream_t st) {
   const dim3 grid((unsigned)a.heads * a.splits * a.batch * a.tiles);
-  const dim3 block(kRows ? 64 : kAttnThreads);
+  const dim3 block(64 * W);
   switch (D == 256 ? 0 : D * 8 + NG) {
-    case 64 * 8 + 1: kv4_attention_kernel<64, 1, C, kRows><<<grid, block, 0, st>>>(a); break;
-    case 64 * 8 + 2: kv4_attention_kernel<64, 2, C, kRows><<<grid, block, 0, st>>>(a); break;
-    case 128 * 8 + 1: kv4_attention_kernel<128, 1, C, kRows><<<grid, block, 0, st>>>(a); break;
-    case 128 * 8 + 2: kv4_attention_kernel<128, 2, C, kRows><<<grid, block, 0, st>>>(a); break;
-    case 128 * 8 + 4: kv4_attention_kernel<128, 4, C, kRows><<<grid, block, 0, st>>>(a); break;
+    case 64 * 8 + 1: kv4_attention_kernel<64, 1, C, W><<<grid, block, 0, st>>>(a); break;
+    case 64 * 8 + 2: kv4_attention_kernel<64, 2, C, W><<<grid, block, 0, st>>>(a); break;
+    case 128 * 8 + 1: kv4_attention_kernel<128, 1, C, W><<<grid, block, 0, st>>>(a); break;
+    case 128 * 8 + 2: kv4_attention_kernel<128, 2, C, W><<<grid, block, 0, st>>>(a); break;
+    case 128 * 8 + 4: kv4_attention_kernel<128, 4, C, W><<<grid, block, 0, st>>>(a); break;
     default:
-      if constexpr (C == 1) {   // (two columns of heads of 256 do not fit the registers)
+      if constexpr (C == 1 && W < 8) {   // (two columns of heads of 256 do not fit the registers,
+                                         // eight waves of them are not used)
         switch (NG) {
-          case 1: kv4_attention_kernel<256, 1, 1, kRows><<<grid, block, 0, st>>>(a); break;
-          case 2: kv4_attention_kernel<256, 2, 1, kRows><<<grid, block, 0, st>>>(a); break;
-          default: kv4_attention_kernel<256, 4, 1, kRows><<<grid, block, 0, st>>>(a); break;
+          case 1: kv4_attention_kernel<256, 1, 1, W><<<grid, block, 0, st>>>(a); break;
+          case 2: kv4_attention_kernel<256, 2, 1, W><<<grid, block, 0, st>>>(a); break;
+          default: kv4_attention_kernel<256, 4, 1, W><<<grid, block, 0, st>>>(a); break;
         }
         break;
       }
@@ -803,6 +809,7 @@ hipError_t launch_attention_form(const AttnArgs& a, int D, int NG, hipStream_t s
   return hipGetLastError();
 }
 hipError_t launch_attention_tokens1(const AttnArgs& a, int D, int NG, hipStream_t st);
+hipError_t launch_attention_tokens1_wide(const AttnArgs& a, int D, int NG, hipStream_t st);
 hipError_t launch_attention_tokens2(const AttnArgs& a, int D, int NG, hipStream_t st);
 hipError_t launch_attention_rows(const AttnArgs& a, int D, int NG, hipStream_t st);
 hipError_t launch_attention_rows256(const AttnArgs& a, int NG, hipStream_t st);

@@ -4,7 +4,7 @@
 namespace w4a16 {
 
 hipError_t launch_attention_tokens2(const AttnArgs& a, int D, int NG, hipStream_t st) {
-  return launch_attention_form<2, false>(a, D, NG, st);
+  return launch_attention_form<2, 4>(a, D, NG, st);
 }
 
 }  // namespace w4a16

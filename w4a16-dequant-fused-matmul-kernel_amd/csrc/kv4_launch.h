@@ -17,19 +17,19 @@ hipError_t launch_kv4_read(const w4a16_kv4& kv, const int32_t* positions, const 
                            int64_t tokens, void* k, void* v, bool bf16, hipStream_t st);
 
 // One attention call, planned (kv4_attention_plan).  A workgroup has 16 * cols query
-// rows; four waves that take 32-token blocks in turn, or (rows_form) one wave that
-// takes all of its range.
+// rows; four waves (wide: eight) that take 32-token blocks in turn, or (rows_form) one
+// wave that takes all of its range.
 // `chunk` blocks of 32 tokens to a split, the last split to the end; splits > 1
 // leave fp32 partials (unnormalised sums, then maximum and denominator) in `part`.
 struct Kv4Attn {
   w4a16_kv4 kv;
   w4a16_kv4_query q;
-  bool rows_form;
+  bool rows_form, wide;
   int cols, tiles, splits, chunk;
   float* part;
 };
 struct Kv4Plan {
-  bool rows_form;
+  bool rows_form, wide;
   int cols, tiles, splits, chunk;
   size_t workspace;
 };

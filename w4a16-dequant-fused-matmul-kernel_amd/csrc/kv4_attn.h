@@ -13,7 +13,7 @@
 // operand of the 32 times 2^-14, each rounded down to it.  The codes stand at 2^-20, so
 // that this is 2^-18 of a code step, times the largest query value or weight of the
 // 32, for those that are much smaller.  (At 2^-24 keys take five instructions, and two
-// prompts 270 us for 278; but one query value 64 times the others moved scores by 4e-4,
+// prompts 8 us less of 278; but one query value 64 times the others moved scores by 4e-4,
 // now by 1e-5, and one-token weights moved results by 5e-5 of a value's range.  Codes
 // less 8 as normal halves for values, and the centres' scores as fma: 289 us.)
 //
@@ -36,7 +36,7 @@
 // MB: 58 us, 4.6 TB/s; one of 1000: 6 us, the latency of a few dependent reads);
 // prompts, vector and matrix instructions together, which hardly overlap on a SIMD
 // (16x16x32 products with four fma each take 10.5 ns among four waves, alone 7.0 and
-// 4.7): 2048 queries on 4000 tokens and 1266 on 2472 take 278 us, 496 TFLOP/s.  Placing
+// 4.7): 2048 queries on 4000 tokens and 1266 on 2472 take 270 us, 511 TFLOP/s.  Placing
 // products between other columns' scores, weights or centres' sums changed nothing.
 // fma with an fp16 operand, packed fp16 and conversions cost 1.6 times a plain fp32
 // instruction.
@@ -123,6 +123,13 @@ __device__ __forceinline__ f16x8 code_halves(uint32_t w) {
   const u32x4 u = {(w << 4) & 0x00F000F0u, w & 0x00F000F0u, (w >> 4) & 0x00F000F0u,
                    (w >> 8) & 0x00F000F0u};
   return __builtin_bit_cast(f16x8, u);
+}
+// (fmaxf would first quiet what might be a signalling NaN, which scores never are: two
+// prompts 278 us with it, 270 without)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
 }
 __device__ __forceinline__ float lo_f32(uint32_t w) { return (float)as_h((uint16_t)w); }
 __device__ __forceinline__ float hi_f32(uint32_t w) { return (float)as_h((uint16_t)(w >> 16)); }
@@ -430,8 +437,8 @@ struct AttnWave {
     bool move = most.x >= limit;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      top[c] = fmaxf(fmaxf(fmaxf(sc[c][0], sc[c][1]), fmaxf(sc[c][2], sc[c][3])),
-                     fmaxf(fmaxf(sc[c][4], sc[c][5]), fmaxf(sc[c][6], sc[c][7])));
+      top[c] = max3(max3(sc[c][0], sc[c][1], sc[c][2]), max3(sc[c][3], sc[c][4], sc[c][5]),
+                    max3(sc[c][6], sc[c][7], sc[c][7]));
       move |= top[c] * fac[c] > ref[c] + room;
     }
     if (__ballot(move)) {
